@@ -23,6 +23,7 @@ FU_SYNC_ENTRY = 8
 FU_SYNC_COUNTER = 32
 FU_SYNC_EPOCH = 33
 FU_SYNC_FAILED = 35
+FU_KV_BLOCK = 64
 FU_FWD_NO_PEER_WAIT = 1
 
 
@@ -47,6 +48,9 @@ STATUS_NAMES = {
     1: "pipeline wait timed out",
     2: "peer flag wait timed out",
     3: "position outside rope_cache",
+    4: "cu_seqlens or seq_lens do not fit the call",
+    5: "slot or block outside the K/V cache",
+    6: "slot named twice in one append",
 }
 
 # FLASH_ULYSSES_B200_LIB points at a library built elsewhere (e.g. a system
@@ -62,6 +66,8 @@ EXPORTED = (
     "fu_qkv_last_grid", "fu_qkv_forward_noalloc",
     "fu_oproj_sync_words", "fu_oproj_create", "fu_oproj_destroy", "fu_oproj_forward",
     "fu_oproj_calls", "fu_oproj_last_grid",
+    "fu_attention_forward", "fu_kvcache_append", "fu_kvcache_attention_workspace",
+    "fu_kvcache_attention",
 )
 
 
@@ -107,6 +113,59 @@ class OprojTopology(ctypes.Structure):
     ]
 
 
+class AttentionArgs(ctypes.Structure):
+    """``fu_attention_args``."""
+
+    _fields_ = [
+        ("device", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("tokens", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64),
+        ("k_stride", ctypes.c_int64),
+        ("v_stride", ctypes.c_int64),
+        ("out_stride", ctypes.c_int64),
+        ("cu_seqlens", ctypes.c_void_p),
+        ("prefix_lens", ctypes.c_void_p),
+        ("alibi_slopes", ctypes.c_void_p),
+        ("docs", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+        ("status_host", ctypes.c_void_p),
+        ("timeout_ns", ctypes.c_uint64),
+    ]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """``fu_kvcache``."""
+
+    _fields_ = [
+        ("device", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("max_seqs", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("reserved0", ctypes.c_int32),
+        ("k_blocks", ctypes.c_void_p),
+        ("v_blocks", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("k_tail", ctypes.c_void_p),
+        ("v_tail", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+    ]
+
+
+address_of = ctypes.addressof
+
+
 def _load():
     if not LIB_PATH.exists():
         raise ImportError(
@@ -139,6 +198,13 @@ def _load():
         "fu_oproj_forward": (ctypes.c_int, [vp, vp, vp, i64, vp, u32, vp]),
         "fu_oproj_calls": (u32, [vp]),
         "fu_oproj_last_grid": (ctypes.c_int, [vp]),
+        "fu_attention_forward": (ctypes.c_int, [vp, u32, vp]),
+        "fu_kvcache_append": (ctypes.c_int, [vp, vp, vp, i64, i64, i64, vp, vp, vp, i32, vp, vp,
+                                             u32, vp]),
+        "fu_kvcache_attention_workspace": (i64, [i32, i32, i32, i32]),
+        "fu_kvcache_attention": (ctypes.c_int, [vp, vp, i64, vp, i64, i32, vp, vp, i32,
+                                                ctypes.c_float, ctypes.c_float, vp, vp, i64, vp,
+                                                vp, u32, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -365,6 +431,41 @@ class OprojOp:
             self.handle = None
 
 
+def attention_forward(device, q_heads, kv_heads, causal, tokens, q, k, v, out, q_stride, k_stride,
+                      v_stride, out_stride, cu_seqlens, prefix_lens, alibi_slopes, docs, scale,
+                      softcap, status, status_host, timeout_ns, flags, stream):
+    """``fu_attention_forward`` on raw device pointers."""
+    if _fast is not None:
+        _fast.attention(device, q_heads, kv_heads, causal, tokens, q, k, v, out, q_stride,
+                        k_stride, v_stride, out_stride, cu_seqlens, prefix_lens, alibi_slopes,
+                        docs, scale, softcap, status, status_host, timeout_ns, flags, stream)
+        return
+    a = AttentionArgs(device, q_heads, kv_heads, causal, tokens, q, k, v, out, q_stride, k_stride,
+                      v_stride, out_stride, cu_seqlens, prefix_lens, alibi_slopes, docs, scale,
+                      softcap, 0, status, status_host, timeout_ns)
+    check(lib.fu_attention_forward(ctypes.byref(a), flags, stream), "fu_attention_forward")
+
+
+def kvcache_append(*args):
+    """``fu_kvcache_append`` on raw device pointers (the header's arguments)."""
+    if _fast is not None:
+        _fast.kvcache_append(*args)
+        return
+    check(lib.fu_kvcache_append(*args), "fu_kvcache_append")
+
+
+def kvcache_attention(*args):
+    """``fu_kvcache_attention`` on raw device pointers (the header's arguments)."""
+    if _fast is not None:
+        _fast.kvcache_attention(*args)
+        return
+    check(lib.fu_kvcache_attention(*args), "fu_kvcache_attention")
+
+
+def kvcache_attention_workspace(device, q_heads, kv_heads, seqs):
+    return int(lib.fu_kvcache_attention_workspace(device, q_heads, kv_heads, seqs))
+
+
 def oproj_sync_words(max_local_tokens):
     return int(lib.fu_oproj_sync_words(max_local_tokens))
 
@@ -383,7 +484,8 @@ def launch(x, qkv_weight, positions, q_gamma, k_gamma, rope, op: QkvOp, *, q_eps
 
 __all__ = [
     "lib", "Topology", "OprojTopology", "ParallelTensor", "StatusWord", "QkvOp", "OprojOp",
-    "oproj_sync_words", "launch", "check",
+    "AttentionArgs", "KvCacheDesc", "attention_forward", "kvcache_append", "kvcache_attention",
+    "kvcache_attention_workspace", "oproj_sync_words", "launch", "check",
     "decode_status", "tensor_from_device_ptr", "EXPORTED", "LIB_PATH",
 ]
 

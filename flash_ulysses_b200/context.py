@@ -21,17 +21,23 @@ keywords, properties, ``ulysses_qkv_forward`` signature, output aliasing and
   queued behind a failed call) stores nothing into any receive buffer and
   waits for no peer.
 
-Added (no counterpart in the reference): with ``output_projection=True``,
-``ulysses_o_proj_forward`` runs the inverse exchange after attention fused with
-the attention output projection.
+Added (no counterpart in the reference): ``ulysses_attention_forward`` is the
+attention over the exchanged rows, ``kv_cache_append`` and
+``kv_cache_attention`` keep an 8-bit K/V cache and attend to it one token per
+sequence, and with ``output_projection=True`` ``ulysses_o_proj_forward`` runs
+the inverse exchange after attention fused with the attention output
+projection.
 """
 
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.distributed as dist
 
 from . import _C
+from .kv_cache import KvCache
 
 
 class FlashUlyssesContext:
@@ -291,6 +297,210 @@ class FlashUlyssesContext:
         stream = _C.current_stream_handle(self.device.index)
         self._oproj.forward(attn_output.data_ptr(), o_proj_weight.data_ptr(), local_tokens,
                             out.data_ptr(), 0, stream)
+        return out
+
+    # ------------------------------------------------------------ attention
+    def _row_stride(self, name, t, rows, heads):
+        """Row stride of a BF16 [rows, heads * 128] tensor; raises on any other."""
+        width = heads * self.head_dim
+        if (t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows
+                or t.shape[1] != width or t.device != self.device):
+            raise ValueError(f"{name} must be a BF16 tensor of shape {(rows, width)} "
+                             f"on {self.device}")
+        row, column = t.stride()
+        if rows == 1:
+            row = width
+        if column != 1 or row < width or row % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be 16-byte aligned with contiguous rows whose stride "
+                             "is a multiple of 8 elements")
+        return row
+
+    def _vector(self, name, t, dtype, length):
+        """Address of a contiguous vector of `length` elements; raises on any other."""
+        if (t.dtype != dtype or t.dim() != 1 or t.shape[0] != length or not t.is_contiguous()
+                or t.device != self.device):
+            raise ValueError(f"{name} must be a contiguous {dtype} vector of {length} elements "
+                             f"on {self.device}")
+        return t.data_ptr()
+
+    def _score_options(self, scale, softcap, alibi_slopes):
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        softcap = float(softcap)
+        if not math.isfinite(scale) or not math.isfinite(softcap) or softcap < 0:
+            raise ValueError("scale must be finite, softcap finite and not negative")
+        slopes = None
+        if alibi_slopes is not None:
+            slopes = self._vector("alibi_slopes", alibi_slopes, torch.float32,
+                                  self.output_q_heads)
+        return scale, softcap, slopes
+
+    def _output(self, out, rows, *inputs):
+        """`out` or a new tensor, and its row stride."""
+        heads = self.output_q_heads
+        if out is None:
+            out = torch.empty(rows, heads * self.head_dim, dtype=torch.bfloat16,
+                              device=self.device)
+            return out, heads * self.head_dim
+        stride = self._row_stride("out", out, rows, heads)
+        begin, end = out.data_ptr(), out.data_ptr() + 2 * ((rows - 1) * stride + out.shape[1])
+        for t in inputs:
+            first = t.data_ptr()
+            last = first + 2 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])
+            if rows and begin < last and first < end:
+                raise ValueError("out must not overlap an input")
+        return out, stride
+
+    def _raise_earlier(self):
+        if self._status.value:
+            raise RuntimeError("an earlier call failed on the device: "
+                               + _C.decode_status(self._status.value))
+
+    @torch.no_grad()
+    def ulysses_attention_forward(self, q, k, v, *, cu_seqlens=None, prefix_lens=None,
+                                  causal=True, scale=None, softcap=0.0, alibi_slopes=None,
+                                  out=None):
+        """Attention over the exchanged rows (no counterpart in the reference).
+
+        ``q`` is BF16 ``[T, output_q_heads * 128]``, ``k`` and ``v`` BF16
+        ``[T, output_kv_heads * 128]``: the layout that ``ulysses_qkv_forward``
+        returns, or any tensors with contiguous, 16-byte aligned rows.  Query
+        head ``h`` reads K/V head ``h // (q heads / kv heads)``.
+
+        ``cu_seqlens`` (int32, ``[documents + 1]``) packs several documents
+        into the rows: document ``d`` is rows ``cu_seqlens[d]`` up to
+        ``cu_seqlens[d + 1]``, and a row sees rows of its own document only.
+        It starts at 0 and does not decrease; rows behind its last entry are
+        neither read nor written.  Without it all rows are one document.
+        ``causal=True`` lets a row see itself and the rows before it, and with
+        ``prefix_lens`` (int32, ``[documents]``, needs ``causal``) also the
+        first ``prefix_lens[d]`` rows of its document.
+
+        Scores are ``scale * q.k`` (default ``128 ** -0.5``), then
+        ``softcap * tanh(score / softcap)`` if ``softcap`` is positive, then
+        less ``alibi_slopes[h] * |i - j|`` if ``alibi_slopes`` (FP32
+        ``[output_q_heads]``, this rank's heads) is given.  Scores and sums are
+        FP32.  Rows that are not seen take no part, whatever they hold.
+
+        Returns BF16 ``[T, output_q_heads * 128]``, the layout that
+        ``ulysses_o_proj_forward`` takes, written into ``out`` when given.
+        Lengths are read on the device, so a captured call may be replayed
+        with other lengths in the same tensors.
+        """
+        rows = q.shape[0]
+        strides = (self._row_stride("q", q, rows, self.output_q_heads),
+                   self._row_stride("k", k, rows, self.output_kv_heads),
+                   self._row_stride("v", v, rows, self.output_kv_heads))
+        if rows > 1 << 30:
+            raise ValueError("at most 2^30 rows")
+        scale, softcap, slopes = self._score_options(scale, softcap, alibi_slopes)
+        docs, cu, prefix = 1, None, None
+        if cu_seqlens is not None:
+            docs = cu_seqlens.numel() - 1
+            cu = self._vector("cu_seqlens", cu_seqlens, torch.int32, max(docs + 1, 1))
+        if prefix_lens is not None:
+            if not causal:
+                raise ValueError("prefix_lens needs causal=True")
+            prefix = self._vector("prefix_lens", prefix_lens, torch.int32, docs)
+        self._raise_earlier()
+        out, out_stride = self._output(out, rows, q, k, v)
+        if rows == 0 or docs == 0:
+            return out
+        index = self.device.index
+        _C.attention_forward(index, self.output_q_heads, self.output_kv_heads, int(bool(causal)),
+                             rows, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                             *strides, out_stride, cu, prefix, slopes, docs, scale, softcap,
+                             self._status.device_ptr, self._status.host_ptr, 0, 0,
+                             _C.current_stream_handle(index))
+        return out
+
+    def create_kv_cache(self, num_blocks, max_seqs, max_blocks):
+        """A zeroed :class:`KvCache` for this rank's K/V heads: ``num_blocks``
+        blocks of 64 tokens, ``max_seqs`` slots, sequences of up to
+        ``max_blocks`` blocks."""
+        return KvCache.allocate(num_blocks, max_seqs, max_blocks, self.output_kv_heads,
+                                self.device)
+
+    def _check_cache(self, cache):
+        if cache.device != self.device or cache.kv_heads != self.output_kv_heads:
+            raise ValueError(f"the cache must hold {self.output_kv_heads} K/V heads "
+                             f"on {self.device}")
+
+    @torch.no_grad()
+    def kv_cache_append(self, cache, k, v, slots, seq_lens, *, cu_seqlens=None):
+        """Write new K/V rows into ``cache`` (no counterpart in the reference).
+
+        ``k`` and ``v`` are BF16 ``[T, output_kv_heads * 128]`` as
+        ``ulysses_qkv_forward`` returns them.  Without ``cu_seqlens`` each row
+        is the next token of one sequence: ``slots`` and ``seq_lens`` (int32,
+        ``[T]``) give its slot in the cache and its length, the new token
+        included.  With ``cu_seqlens`` (int32, ``[n + 1]``, from 0, not
+        decreasing) rows ``cu_seqlens[i]`` up to ``cu_seqlens[i + 1]`` are the
+        next tokens of slot ``slots[i]``, whose length becomes ``seq_lens[i]``
+        (both ``[n]``); rows behind its last entry are not read.
+
+        A negative slot is skipped, so a batch may be padded.  Blocks that the
+        call completes are written to ``cache.block_table``'s blocks in 8 bits;
+        the rest stays in the slot's tail.  A slot may occur only once in a
+        call.  Slots, blocks or lengths that do not fit the cache are reported
+        like every device-side error, by the next call or ``check()``, and
+        nothing is written for them.
+        """
+        rows, count = k.shape[0], slots.numel()
+        k_stride = self._row_stride("k", k, rows, self.output_kv_heads)
+        v_stride = self._row_stride("v", v, rows, self.output_kv_heads)
+        self._check_cache(cache)
+        if rows > 1 << 30 or count > 1 << 24:
+            raise ValueError("at most 2^30 rows and 2^24 sequences")
+        slot_ptr = self._vector("slots", slots, torch.int32, count if cu_seqlens is not None
+                                else rows)
+        lens_ptr = self._vector("seq_lens", seq_lens, torch.int32, count)
+        cu = None
+        if cu_seqlens is not None:
+            cu = self._vector("cu_seqlens", cu_seqlens, torch.int32, count + 1)
+        self._raise_earlier()
+        if rows == 0 or count == 0:
+            return
+        _C.kvcache_append(cache._address, k.data_ptr(), v.data_ptr(), k_stride, v_stride, rows,
+                          slot_ptr, lens_ptr, cu, count, self._status.device_ptr,
+                          self._status.host_ptr, 0, _C.current_stream_handle(self.device.index))
+
+    @torch.no_grad()
+    def kv_cache_attention(self, cache, q, slots, seq_lens, *, scale=None, softcap=0.0,
+                           alibi_slopes=None, out=None):
+        """Attention of one token per sequence over ``cache`` (no counterpart
+        in the reference).
+
+        ``q`` is BF16 ``[n, output_q_heads * 128]``, row ``i`` the last token of
+        the sequence in slot ``slots[i]``, which attends to that sequence's
+        first ``seq_lens[i]`` tokens (int32 ``[n]`` each), so append it first.
+        Scores as in ``ulysses_attention_forward``.  Returns BF16
+        ``[n, output_q_heads * 128]``, written into ``out`` when given.  A row
+        with a negative slot is left as it was, one with length 0 is zeroed; a
+        slot may occur more than once.  Slots, blocks and lengths that do not
+        fit the cache are reported by the next call or ``check()``.
+        """
+        rows = q.shape[0]
+        q_stride = self._row_stride("q", q, rows, self.output_q_heads)
+        self._check_cache(cache)
+        if rows > 1 << 24:
+            raise ValueError("at most 2^24 sequences")
+        slot_ptr = self._vector("slots", slots, torch.int32, rows)
+        lens_ptr = self._vector("seq_lens", seq_lens, torch.int32, rows)
+        scale, softcap, slopes = self._score_options(scale, softcap, alibi_slopes)
+        self._raise_earlier()
+        out, out_stride = self._output(out, rows, q)
+        if rows == 0:
+            return out
+        index = self.device.index
+        # Scratch from torch's allocator, so calls on other streams and captured
+        # graphs each have their own.
+        nbytes = _C.kvcache_attention_workspace(index, self.output_q_heads,
+                                                self.output_kv_heads, rows)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        _C.kvcache_attention(cache._address, q.data_ptr(), q_stride, out.data_ptr(), out_stride,
+                             self.output_q_heads, slot_ptr, lens_ptr, rows, scale, softcap,
+                             slopes, work.data_ptr(), nbytes, self._status.device_ptr,
+                             self._status.host_ptr, 0, _C.current_stream_handle(index))
         return out
 
     def check(self):

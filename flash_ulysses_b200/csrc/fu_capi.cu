@@ -45,19 +45,6 @@ EncodeTiledFn encode_tiled_fn() {
 }
 
 namespace {
-struct DeviceGuard {
-    int prev = -1;
-    bool changed = false;
-    explicit DeviceGuard(int device) {
-        if (cudaGetDevice(&prev) == cudaSuccess && prev != device) {
-            changed = cudaSetDevice(device) == cudaSuccess;
-        }
-    }
-    ~DeviceGuard() {
-        if (changed) cudaSetDevice(prev);
-    }
-};
-
 int cuda_fail(const char* what, cudaError_t e) {
     return set_error(FU_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }

@@ -74,6 +74,9 @@ enum : int32_t {
     FU_DEV_PIPELINE_TIMEOUT = 1,
     FU_DEV_PEER_TIMEOUT = 2,
     FU_DEV_POSITION_RANGE = 3,
+    FU_DEV_LENGTHS = 4,
+    FU_DEV_CACHE_RANGE = 5,
+    FU_DEV_SLOT_TWICE = 6,
 };
 
 __device__ __forceinline__ void report_status(int32_t* status, int32_t code, int32_t where) {

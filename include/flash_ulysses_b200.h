@@ -76,7 +76,10 @@ enum fu_device_status {
     FU_STATUS_OK = 0,
     FU_STATUS_PIPELINE_TIMEOUT = 1,
     FU_STATUS_PEER_TIMEOUT = 2,
-    FU_STATUS_POSITION_RANGE = 3
+    FU_STATUS_POSITION_RANGE = 3,
+    FU_STATUS_LENGTHS = 4,         /* cu_seqlens or seq_lens that do not fit the call */
+    FU_STATUS_CACHE_RANGE = 5,     /* a slot or block index outside the K/V cache */
+    FU_STATUS_SLOT_TWICE = 6       /* a slot named twice in one append */
 };
 
 /* Default bound on a device-side wait: 30 s, long enough for ranks whose
@@ -312,6 +315,128 @@ FU_API int fu_oproj_forward(fu_oproj_ctx* ctx, const void* attn, const void* w_o
 FU_API uint32_t fu_oproj_calls(const fu_oproj_ctx* ctx);
 /* Number of CTAs the most recent call launched. */
 FU_API int fu_oproj_last_grid(const fu_oproj_ctx* ctx);
+
+/* ------------------------------------------------------------------------
+ * Attention over the exchanged rows.  No counterpart in the reference, whose
+ * outputs feed it: fu_qkv_forward delivers Q, K and V of this rank's heads for
+ * the whole group's sequence, this turns them into the rows that
+ * fu_oproj_forward takes.
+ *
+ * Rows are packed documents: row i of document d = [cu_seqlens[d],
+ * cu_seqlens[d+1]) sees the rows [lo, hi) of its own document, lo the
+ * document's start and hi its end, or with causal
+ *     hi = max(i + 1, lo + prefix_lens[d])
+ * (a prefix is read in both directions).  For query head h and its K/V head
+ * h / (q_heads / kv_heads), over the rows j seen:
+ *     x_ij  = scale * q_i . k_j
+ *     x_ij  = softcap * tanh(x_ij / softcap)      if softcap > 0
+ *     x_ij -= alibi_slopes[h] * |i - j|           if alibi_slopes
+ *     out_i = sum_j softmax_j(x_ij) v_j
+ * Scores, softmax and sums are FP32; the weights are rounded to BF16 for the
+ * second product and the output is rounded to BF16.  Rows that are not seen
+ * take no part, whatever they hold (infinities and NaN included).  Rows
+ * behind cu_seqlens[docs] are left as they were.  cu_seqlens starts at 0, does
+ * not decrease and ends at tokens or less (empty documents are allowed); what
+ * does not is reported as FU_STATUS_LENGTHS, with results undefined.
+ * ------------------------------------------------------------------------ */
+typedef struct fu_attention_args {
+    int32_t device;
+    int32_t q_heads;              /* a multiple of kv_heads */
+    int32_t kv_heads;
+    int32_t causal;
+    int64_t tokens;               /* rows of q, k, v and out: 1 .. 2^30 */
+    /* BF16, 16-byte aligned, row r at r * stride elements (a multiple of 8). */
+    const void* q;                /* [tokens, q_heads * 128] */
+    const void* k;                /* [tokens, kv_heads * 128] */
+    const void* v;                /* [tokens, kv_heads * 128] */
+    void* out;                    /* [tokens, q_heads * 128] */
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    const int32_t* cu_seqlens;    /* device, [docs + 1], or NULL: one document of all rows */
+    const int32_t* prefix_lens;   /* device, [docs], or NULL; with causal only */
+    const float* alibi_slopes;    /* device, [q_heads], or NULL */
+    int32_t docs;                 /* documents: 1 .. 2^30 (1 without cu_seqlens) */
+    float scale;
+    float softcap;                /* 0: scores are not capped */
+    int32_t reserved0;
+    int32_t* status;              /* as in fu_qkv_topology, may be NULL */
+    int32_t* status_host;
+    uint64_t timeout_ns;          /* bound on every device-side wait; 0 = FU_DEFAULT_TIMEOUT_NS */
+} fu_attention_args;
+
+/* One call, one launch on `stream` (flags: FU_FWD_NO_PDL).  Allocates nothing
+ * and keeps nothing. */
+FU_API int fu_attention_forward(const fu_attention_args* args, uint32_t flags, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A K/V cache held in 8 bits, and the attention of single tokens that reads
+ * it.  No counterpart in the reference.
+ *
+ * Every full block of FU_KV_BLOCK tokens of a K/V head is held in e4m3 with
+ * one FP32 scale, the smallest power of two from 2^-126 up that brings the
+ * block's largest finite value to 448 or less; value = e4m3 * scale, rounded
+ * to nearest even (infinities and NaN become NaN).  The last, unfinished block
+ * of each sequence is held in BF16, so each token is rounded once, with its
+ * whole block known: the cache does not depend on how the tokens were split
+ * into calls.
+ *
+ * A sequence has a slot (its row of block_table and of the tails); its block
+ * b of 64 tokens is cache block block_table[slot][b].  Blocks and table are
+ * the caller's to assign.  seq_lens[i] counts the tokens of batch row i's
+ * sequence, those of the call included.
+ * ------------------------------------------------------------------------ */
+#define FU_KV_BLOCK 64
+
+typedef struct fu_kvcache {
+    int32_t device;
+    int32_t kv_heads;
+    int32_t num_blocks;
+    int32_t max_seqs;             /* slots */
+    int32_t max_blocks;           /* columns of block_table; max_blocks * 64 < 2^31 */
+    int32_t reserved0;
+    void* k_blocks;               /* e4m3 [num_blocks, kv_heads, 64 tokens, 128] */
+    void* v_blocks;               /* e4m3 [num_blocks, kv_heads, 128, 64 tokens] */
+    float* k_scales;              /* [num_blocks, kv_heads] */
+    float* v_scales;
+    void* k_tail;                 /* BF16 [max_seqs, kv_heads, 64, 128] */
+    void* v_tail;
+    const int32_t* block_table;   /* [max_seqs, max_blocks] */
+} fu_kvcache;
+
+/* Write new rows k, v (BF16 [tokens, kv_heads * 128], 16-byte aligned, row
+ * strides in elements, multiples of 8) behind their sequences, as the places
+ * seq_lens[i] - n_i .. seq_lens[i] - 1 of slot slots[i].  Without cu_seqlens
+ * n_i = 1 and row i belongs to slots[i] (tokens == seqs); with it the rows of
+ * sequence i are [cu_seqlens[i], cu_seqlens[i + 1]) (seqs + 1 device words,
+ * from 0, not decreasing, up to tokens).  slots and seq_lens are device
+ * int32 [seqs].  A negative slot is skipped (a padded batch).  Skipped and
+ * reported: a slot that an earlier row names too (FU_STATUS_SLOT_TWICE), a
+ * slot or block outside the cache (FU_STATUS_CACHE_RANGE), a length below n_i
+ * or above max_blocks * 64, or rows that cu_seqlens puts outside the call
+ * (FU_STATUS_LENGTHS). */
+FU_API int fu_kvcache_append(const fu_kvcache* cache, const void* k, const void* v,
+                             int64_t k_stride, int64_t v_stride, int64_t tokens,
+                             const int32_t* slots, const int32_t* seq_lens,
+                             const int32_t* cu_seqlens, int32_t seqs, int32_t* status,
+                             int32_t* status_host, uint32_t flags, void* stream);
+
+/* Scratch bytes of fu_kvcache_attention.  The scratch holds no state between
+ * calls; calls that may run at the same time need one each. */
+FU_API int64_t fu_kvcache_attention_workspace(int32_t device, int32_t q_heads, int32_t kv_heads,
+                                              int32_t seqs);
+
+/* out_i = attention of row i's query heads over the first seq_lens[i] tokens
+ * of slot slots[i], the query being the last of them; scores as in
+ * fu_attention_forward.  q and out are BF16 [seqs, q_heads * 128] with row
+ * strides.  A row whose slot is negative is left as it was, one whose length
+ * is 0 is zeroed.  A slot may occur more than once.  A slot outside the cache
+ * or a length outside [0, max_blocks * 64] is reported and its row left as it
+ * was; the keys of a block outside the cache are reported and not seen. */
+FU_API int fu_kvcache_attention(const fu_kvcache* cache, const void* q, int64_t q_stride,
+                                void* out, int64_t out_stride, int32_t q_heads,
+                                const int32_t* slots, const int32_t* seq_lens, int32_t seqs,
+                                float scale, float softcap, const float* alibi_slopes,
+                                void* workspace, int64_t workspace_bytes, int32_t* status,
+                                int32_t* status_host, uint32_t flags, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,333 @@
+"""Host side of the attention and cache operators without a GPU: the refusals of every argument,
+the cache's own checks, the layout of the C structures, and the append's work units."""
+
+import ctypes
+import random
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from flash_ulysses_b200 import FlashUlyssesContext, KvCache, _C
+
+ROOT = Path(__file__).resolve().parent.parent
+HEADER = ROOT / "include" / "flash_ulysses_b200.h"
+BF16, I32, F32 = torch.bfloat16, torch.int32, torch.float32
+
+
+class NoStatus:
+    value = 0
+    device_ptr = host_ptr = None
+
+
+@pytest.fixture
+def ctx(monkeypatch):
+    """A context of 4 query and 2 K/V heads whose tensors are on the CPU; a launch fails."""
+    c = object.__new__(FlashUlyssesContext)
+    c.world_size, c.sp_size, c.num_heads, c.num_kv_heads, c.head_dim = 1, 1, 4, 2, 128
+    c.device, c._status = torch.device("cpu"), NoStatus()
+
+    def launched(*args):
+        raise AssertionError("launched")
+
+    for name in ("attention_forward", "kvcache_append", "kvcache_attention"):
+        monkeypatch.setattr(_C, name, launched)
+    monkeypatch.setattr(_C, "current_stream_handle", lambda index: 0)
+    monkeypatch.setattr(_C, "kvcache_attention_workspace", lambda *sizes: 16)
+    return c
+
+
+def q_k_v(n=6):
+    return (torch.zeros(n, 512, dtype=BF16), torch.zeros(n, 256, dtype=BF16),
+            torch.zeros(n, 256, dtype=BF16))
+
+
+def test_attention_reaches_the_launch(ctx):
+    q, k, v = q_k_v()
+    cu, pre = torch.tensor([0, 6], dtype=I32), torch.zeros(1, dtype=I32)
+    for extra in ({}, dict(cu_seqlens=cu), dict(cu_seqlens=cu, prefix_lens=pre),
+                  dict(prefix_lens=pre), dict(alibi_slopes=torch.zeros(4)), dict(softcap=30),
+                  dict(out=torch.zeros(6, 512, dtype=BF16)), dict(scale=0.5, causal=False)):
+        with pytest.raises(AssertionError, match="launched"):
+            ctx.ulysses_attention_forward(q, k, v, **extra)
+    packed = torch.zeros(6, 1024, dtype=BF16)
+    with pytest.raises(AssertionError, match="launched"):
+        ctx.ulysses_attention_forward(packed[:, :512], packed[:, 512:768], packed[:, 768:])
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=torch.zeros(6, 256, dtype=BF16)), dict(q=torch.zeros(6, 512)),
+    dict(q=torch.zeros(6, 4, 128, dtype=BF16)), dict(k=torch.zeros(5, 256, dtype=BF16)),
+    dict(v=torch.zeros(6, 512, dtype=BF16)), dict(v=torch.zeros(256, 6, dtype=BF16).t()),
+    dict(q=torch.zeros(6, 516, dtype=BF16)[:, :512]), dict(k=torch.zeros(6, 264, dtype=BF16)[:, 4:260]),
+    dict(q=torch.zeros(1, 512, dtype=BF16).expand(6, 512)),
+    dict(cu_seqlens=torch.zeros(3)), dict(cu_seqlens=torch.zeros(3, dtype=torch.int64)),
+    dict(cu_seqlens=torch.zeros(0, dtype=I32)), dict(cu_seqlens=torch.zeros(6, dtype=I32)[::2]),
+    dict(cu_seqlens=torch.zeros(3, dtype=I32), prefix_lens=torch.zeros(1, dtype=I32)),
+    dict(prefix_lens=torch.zeros(1, dtype=I32), causal=False),
+    dict(prefix_lens=torch.zeros(2, dtype=I32)),
+    dict(alibi_slopes=torch.zeros(2)), dict(alibi_slopes=torch.zeros(4, dtype=BF16)),
+    dict(softcap=-1.0), dict(softcap=float("nan")), dict(scale=float("inf")),
+    dict(out=torch.zeros(6, 512)), dict(out=torch.zeros(5, 512, dtype=BF16)),
+])
+def test_attention_refuses(ctx, change):
+    q, k, v = q_k_v()
+    given = dict(q=q, k=k, v=v)
+    given.update(change)
+    with pytest.raises(ValueError):
+        ctx.ulysses_attention_forward(given.pop("q"), given.pop("k"), given.pop("v"), **given)
+
+
+def test_attention_refuses_output_over_an_input(ctx):
+    q, k, v = q_k_v()
+    with pytest.raises(ValueError, match="overlap"):
+        ctx.ulysses_attention_forward(q, k, v, out=q)
+    packed = torch.zeros(6, 1024, dtype=BF16)
+    with pytest.raises(ValueError, match="overlap"):
+        ctx.ulysses_attention_forward(q, packed[:, 512:768], v, out=packed[:, :512])
+
+
+def test_nothing_to_do(ctx):
+    """No rows, no documents, no sequences: no launch."""
+    q, k, v = q_k_v(0)
+    assert ctx.ulysses_attention_forward(q, k, v).shape == (0, 512)
+    q, k, v = q_k_v(3)
+    out = torch.ones(3, 512, dtype=BF16)
+    none = torch.zeros(0, dtype=I32)
+    assert ctx.ulysses_attention_forward(q, k, v, cu_seqlens=torch.zeros(1, dtype=I32),
+                                         out=out) is out
+    cache = KvCache.allocate(3, 2, 2, 2, "cpu")
+    ctx.kv_cache_append(cache, k[:0], v[:0], none, none)
+    ctx.kv_cache_append(cache, k, v, none, none, cu_seqlens=torch.zeros(1, dtype=I32))
+    assert ctx.kv_cache_attention(cache, q[:0], none, none).shape == (0, 512)
+
+
+def test_earlier_device_error_is_raised(ctx):
+    ctx._status = NoStatus()
+    ctx._status.value = 5 | (80 << 8)
+    q, k, v = q_k_v()
+    cache = KvCache.allocate(3, 2, 2, 2, "cpu")
+    i = torch.zeros(6, dtype=I32)
+    for call in (lambda: ctx.ulysses_attention_forward(q, k, v),
+                 lambda: ctx.kv_cache_append(cache, k, v, i, i),
+                 lambda: ctx.kv_cache_attention(cache, q, i, i)):
+        with pytest.raises(RuntimeError, match="outside the K/V cache"):
+            call()
+
+
+# ------------------------------------------------------------------ cache
+def parts(**change):
+    c = KvCache.allocate(5, 3, 4, 2, "cpu")
+    given = {n: getattr(c, n) for n in ("k_blocks", "v_blocks", "k_scales", "v_scales", "k_tail",
+                                        "v_tail", "block_table")}
+    given.update(change)
+    return given
+
+
+def test_cache_sizes_and_description():
+    c = KvCache.allocate(5, 3, 4, 2, "cpu")
+    assert (c.num_blocks, c.max_seqs, c.max_blocks, c.kv_heads) == (5, 3, 4, 2)
+    assert c.k_blocks.shape == (5, 2, 64, 128) and c.v_blocks.shape == (5, 2, 128, 64)
+    assert c._desc.v_tail == c.v_tail.data_ptr() and c._desc.max_blocks == 4
+    assert c._address == ctypes.addressof(c._desc)
+    again = KvCache(**parts())
+    assert again.kv_heads == 2
+
+
+@pytest.mark.parametrize("change", [
+    dict(k_blocks=torch.zeros(5, 2, 64, 128, dtype=torch.uint8)),
+    dict(v_blocks=torch.zeros(5, 2, 64, 128, dtype=torch.uint8).view(torch.float8_e4m3fn)),
+    dict(k_scales=torch.zeros(5, 3)), dict(v_scales=torch.zeros(5, 2, dtype=BF16)),
+    dict(k_tail=torch.zeros(2, 2, 64, 128, dtype=BF16)),
+    dict(v_tail=torch.zeros(3, 2, 128, 64, dtype=BF16).transpose(2, 3)),
+    dict(block_table=torch.zeros(3, 4, dtype=torch.int64)),
+    dict(block_table=torch.zeros(2, 4, dtype=I32)),
+    dict(block_table=torch.zeros(4, 3, dtype=I32).t()),
+    dict(block_table=torch.zeros(12, dtype=I32)),
+    dict(block_table=torch.zeros(13, dtype=I32)[1:].view(3, 4)),
+])
+def test_cache_refuses(change):
+    with pytest.raises(ValueError):
+        KvCache(**parts(**change))
+
+
+def test_cache_refuses_empty_and_huge():
+    with pytest.raises(ValueError):
+        KvCache.allocate(0, 3, 4, 2, "cpu")
+    with pytest.raises(ValueError):
+        KvCache.allocate(1, 1, 1 << 25, 1, "cpu")
+
+
+def test_append_and_decode_reach_the_launch(ctx):
+    cache = KvCache.allocate(5, 3, 4, 2, "cpu")
+    q, k, v = q_k_v()
+    i = torch.zeros(6, dtype=I32)
+    for call in (lambda: ctx.kv_cache_append(cache, k, v, i, i),
+                 lambda: ctx.kv_cache_append(cache, k, v, i[:2], i[:2],
+                                             cu_seqlens=torch.tensor([0, 2, 6], dtype=I32)),
+                 lambda: ctx.kv_cache_attention(cache, q, i, i, softcap=3.0,
+                                                alibi_slopes=torch.zeros(4))):
+        with pytest.raises(AssertionError, match="launched"):
+            call()
+
+
+@pytest.mark.parametrize("call", [
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, k, v[:5], i, i),
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, q, v, i, i),
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, k, v, i[:5], i[:5]),
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, k, v, i, i[:5]),
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, k, v, i.long(), i),
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, k, v, i, i.float()),
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, k, v, i[:2], i[:2], cu_seqlens=i[:2]),
+    lambda c, a, q, k, v, i: c.kv_cache_append(a, k, v, i.view(2, 3), i),
+    lambda c, a, q, k, v, i: c.kv_cache_append(KvCache.allocate(5, 3, 4, 4, "cpu"), k, v, i, i),
+    lambda c, a, q, k, v, i: c.kv_cache_append(KvCache.allocate(5, 3, 4, 2, "meta"), k, v, i, i),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, k, i, i),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, q.float(), i, i),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, q, i[:5], i),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, q, i, i[:5]),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, q, i, i, softcap=-2.0),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, q, i, i, alibi_slopes=torch.zeros(2)),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, q, i, i, out=q),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(a, q, i, i, out=q[:5].clone()),
+    lambda c, a, q, k, v, i: c.kv_cache_attention(KvCache.allocate(5, 3, 4, 1, "cpu"), q, i, i),
+])
+def test_append_and_decode_refuse(ctx, call):
+    cache = KvCache.allocate(5, 3, 4, 2, "cpu")
+    q, k, v = q_k_v()
+    with pytest.raises(ValueError):
+        call(ctx, cache, q, k, v, torch.zeros(6, dtype=I32))
+
+
+# ------------------------------------------------------------------ C ABI
+def test_struct_layouts_match_the_header(tmp_path):
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    lines = []
+    for cls, name in ((_C.AttentionArgs, "fu_attention_args"), (_C.KvCacheDesc, "fu_kvcache")):
+        lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
+        for field, *_ in cls._fields_:
+            lines.append(f'printf("{name}.{field} %zu\\n", offsetof({name}, {field}));')
+    src = tmp_path / "probe.c"
+    src.write_text('#include <stdio.h>\n#include "flash_ulysses_b200.h"\nint main(void) {\n'
+                   + "\n".join(lines) + "\nreturn 0;\n}\n")
+    exe = tmp_path / "probe"
+    subprocess.run([gcc, "-I", str(HEADER.parent), str(src), "-o", str(exe)], check=True)
+    got = dict(line.split() for line in subprocess.run(
+        [str(exe)], capture_output=True, text=True, check=True).stdout.splitlines())
+    for cls, name in ((_C.AttentionArgs, "fu_attention_args"), (_C.KvCacheDesc, "fu_kvcache")):
+        assert int(got[name]) == ctypes.sizeof(cls)
+        for field, *_ in cls._fields_:
+            assert int(got[f"{name}.{field}"]) == getattr(cls, field).offset, field
+
+
+def test_constants_and_status_codes_match_the_header():
+    text = HEADER.read_text()
+    assert int(re.search(r"#define FU_KV_BLOCK (\d+)", text).group(1)) == _C.FU_KV_BLOCK
+    for name, code, word in (("LENGTHS", 4, "cu_seqlens"), ("CACHE_RANGE", 5, "block"),
+                             ("SLOT_TWICE", 6, "twice")):
+        assert re.search(rf"FU_STATUS_{name} = {code}\b", text)
+        assert word in _C.decode_status(code)
+
+
+def args(**change):
+    a = _C.AttentionArgs()
+    a.q_heads, a.kv_heads, a.tokens, a.docs, a.causal, a.scale = 4, 2, 6, 1, 1, 0.1
+    a.q = a.k = a.v = a.out = 4096
+    a.q_stride = a.out_stride = 512
+    a.k_stride = a.v_stride = 256
+    for n, x in change.items():
+        setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(q_heads=3), dict(kv_heads=0), dict(tokens=0), dict(tokens=(1 << 30) + 1), dict(docs=0),
+    dict(docs=2), dict(causal=0, prefix_lens=4096), dict(softcap=-1.0), dict(scale=float("nan")),
+    dict(q=None), dict(out=4098), dict(k=4104), dict(q_stride=504), dict(v_stride=260),
+])
+def test_c_attention_refuses(change):
+    """Refused on the host, before any CUDA call."""
+    rc = _C.lib.fu_attention_forward(ctypes.byref(args(**change)), 0, None)
+    assert rc == _C.FU_ERR_INVALID and _C.last_error()
+    assert _C.lib.fu_attention_forward(None, 0, None) == _C.FU_ERR_INVALID
+
+
+def description(**change):
+    d = _C.KvCacheDesc()
+    d.kv_heads, d.num_blocks, d.max_seqs, d.max_blocks = 2, 5, 3, 4
+    for n in ("k_blocks", "v_blocks", "k_scales", "v_scales", "k_tail", "v_tail", "block_table"):
+        setattr(d, n, 4096)
+    for n, x in change.items():
+        setattr(d, n, x)
+    return d
+
+
+@pytest.mark.parametrize("cache,change", [
+    (dict(kv_heads=0), {}), (dict(max_blocks=1 << 25), {}), (dict(k_tail=None), {}),
+    (dict(v_blocks=4104), {}), ({}, dict(tokens=5)), ({}, dict(tokens=0)), ({}, dict(seqs=0)),
+    ({}, dict(k=None)), ({}, dict(k_stride=128)), ({}, dict(slots=None)),
+    ({}, dict(seq_lens=None)),
+])
+def test_c_append_refuses(cache, change):
+    d = description(**cache)
+    a = dict(k=4096, v=4096, k_stride=256, v_stride=256, tokens=6, slots=4096, seq_lens=4096,
+             cu=None, seqs=6)
+    a.update(change)
+    rc = _C.lib.fu_kvcache_append(ctypes.addressof(d), *a.values(), None, None, 0, None)
+    assert rc == _C.FU_ERR_INVALID and _C.last_error()
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=None), dict(q_stride=256), dict(out=4100), dict(q_heads=3), dict(seqs=0),
+    dict(slots=None), dict(softcap=-1.0), dict(work=None), dict(nbytes=0),
+])
+def test_c_decode_refuses(change):
+    d = description()
+    a = dict(q=4096, q_stride=512, out=4096, out_stride=512, q_heads=4, slots=4096, seq_lens=4096,
+             seqs=6, scale=0.1, softcap=0.0, slopes=None, work=4096, nbytes=1 << 40)
+    a.update(change)
+    rc = _C.lib.fu_kvcache_attention(ctypes.addressof(d), *a.values(), None, None, 0, None)
+    assert rc == _C.FU_ERR_INVALID and _C.last_error()
+    assert _C.lib.fu_kvcache_attention_workspace(0, 3, 2, 1) == 0
+    assert _C.lib.fu_kvcache_attention_workspace(0, 4, 2, 0) == 0
+
+
+# ------------------------------------------------------------------ append units
+def unit_base(first_row, i):
+    return first_row // 64 + 2 * i
+
+
+def test_append_units_cover_every_block():
+    """Each sequence's units (from its row offset and index alone) are enough for every block its
+    rows can touch, wherever in a block they start, and the grid is enough for all."""
+    rng = random.Random(0)
+    for _ in range(2000):
+        news = [rng.choice([0, 1, 2, 62, 63, 64, 65, 127, 128, 129, rng.randrange(1000)])
+                for _ in range(rng.randrange(1, 20))]
+        cu = [0]
+        for n in news:
+            cu.append(cu[-1] + n)
+        tokens = cu[-1] + rng.choice([0, 1, 100])
+        grid = unit_base(tokens, len(news))
+        for i, n in enumerate(news):
+            first, after = unit_base(cu[i], i), unit_base(cu[i + 1], i + 1)
+            assert after <= grid
+            for start in range(64):
+                touched = (start + n - 1) // 64 + 1 if n else 0
+                assert touched <= after - first
+        # The kernel's search: the last sequence whose units start at or before the unit.
+        for unit in range(grid):
+            a, b = 0, len(news)
+            while b - a > 1:
+                mid = (a + b) // 2
+                if unit_base(cu[mid], mid) <= unit:
+                    a = mid
+                else:
+                    b = mid
+            assert unit_base(cu[a], a) <= unit
+            assert a == len(news) - 1 or unit < unit_base(cu[a + 1], a + 1)
