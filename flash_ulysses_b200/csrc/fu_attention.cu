@@ -1,13 +1,40 @@
 // Attention over the exchanged Q/K/V rows (sm_100a): packed documents, causal,
 // prefix or full masks, scores capped by a tanh and/or lowered with distance.
 //
-// One warp per (row, query head): lane l holds dims 4l..4l+3 of q, of the
-// running output and of each key's k and v; scores by a warp sum, with the
-// running maximum m and sum l of an online softmax in FP32.
+// A CTA computes one query head's 256 rows as two tiles of 128, and walks the
+// keys that any of its rows sees in tiles of 128 with an online softmax:
+//     S = Q K^T          tcgen05, Q and K from shared memory, S in TMEM
+//     m' = max(m, S), P = 2^(c S - c m'), l = l 2^(c m - c m') + sum P
+//     O = O 2^(c m - c m') + P V     tcgen05, P from TMEM, V from shared memory
+// c = scale * log2(e); out = O / l.  A thread of the softmax owns one row, so
+// the maximum and the sum need no exchange between threads.
+//
+// 384 threads: warps 0-3 and 4-7 the softmax of tile 0 and tile 1, warp 8 the
+// TMA loads, warp 9 the MMA issue (and TMEM), warps 10-11 clean V tiles at the
+// edge of a mask (below).  While one tile's scores go through its softmax the
+// tensor cores work on the other tile.
+//
+// TMEM (512 columns): S0, S1, O0, O1, 128 columns each; P, two BF16 per
+// column, overwrites the first 64 columns of its tile's S.  The tile's next S
+// is issued behind the product that reads P, so when S arrives that product
+// is complete too and the softmax warps may rescale O in place.  They do so
+// only when a row's maximum has grown by more than 2^8 (the reference m may
+// lag behind the maximum: P and l stay far inside FP32's and BF16's range),
+// which happens in the first tiles of a row and hardly ever after.
+//
+// Masks: row i sees keys [lo_i, hi_i), both nondecreasing in i, so a tile of
+// rows needs the keys [lo_first, hi_last) and only key tiles that cross a
+// row's lo or hi apply a mask.  In those a key may be hidden from some rows
+// while its V row holds infinities or NaN, and 0 * NaN would reach rows that
+// do not see it: warps 10-11 replace what is not finite by 0 in shared memory
+// before the product, and if they found any, the epilogue adds it back for the
+// rows that see it.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -19,26 +46,56 @@ namespace fu {
 namespace attention {
 
 constexpr int D = FU_HEAD_DIM;
-constexpr int WARPS = 4;
+constexpr int TILE = 128;                       // rows of a query tile, keys of a key tile
+constexpr int ROWS = 2 * TILE;                  // query rows per CTA
+constexpr int NUM_THREADS = 384;
+constexpr int TILE_BYTES = TILE * D * 2;        // 32 KiB: two 64-column boxes
+constexpr int BOX_BYTES = TILE_BYTES / 2;
+constexpr int STAGES = 5;                       // K and V tiles in turn
+constexpr int OFF_Q = 0;
+constexpr int OFF_KV = OFF_Q + 2 * TILE_BYTES;
+constexpr int OFF_SEEN = OFF_KV + STAGES * TILE_BYTES;      // int2[2][2]
+constexpr int OFF_BAR = OFF_SEEN + 64;
+constexpr int OFF_MISC = OFF_BAR + 8 * 32;
+constexpr int SMEM_BYTES = OFF_MISC + 64;
+constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;   // room to align the base to 1 KiB
+static_assert(SMEM_ALLOC <= 232448, "exceeds the 227 KiB per-CTA shared memory limit");
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t TM_S = 0, TM_O = 256;        // + 128 * tile
+// Registers: 3 warpgroups launch with 168 each; the softmax takes 224, the
+// others keep 56 (224 + 224 + 56 = 3 * 168).
+constexpr int SOFTMAX_REGS = 224, OTHER_REGS = 56;
+constexpr float LOG2E = 1.4426950408889634f;
 
 // Status "where" codes of this kernel.
-enum : int { W_CU_SEQLENS = 64 };
+enum : int {
+    W_CU_SEQLENS = 64, W_Q = 65, W_KV_FULL = 66, W_KV_EMPTY = 67, W_S = 68, W_P = 69, W_O = 70,
+    W_CLEAN = 71, W_DRAIN = 72,
+};
 
 struct Params {
-    const __nv_bfloat16* q;
-    const __nv_bfloat16* k;
+    CUtensorMap tm_q, tm_k, tm_v;      // [tokens, heads * 128], box {64, 128}, 128-byte swizzle
     const __nv_bfloat16* v;
     __nv_bfloat16* out;
-    int64_t q_stride, k_stride, v_stride, out_stride;
+    int64_t v_stride, out_stride;
     const int32_t* cu_seqlens;
     const int32_t* prefix_lens;
     const float* alibi_slopes;
     int32_t* status;
-    int32_t tokens, docs, group, causal;
+    unsigned long long timeout_ns;
+    int32_t tokens, docs, q_heads, group, causal;
+    uint32_t negate;                   // scale < 0: the MMA negates Q, `scale` is positive
     float scale, softcap;
 };
 
-// Rows [lo, hi) that row i sees; empty for a row behind the last document.
+struct Bars {
+    uint32_t q, kv_full, kv_empty, s, p, o, done, clean;
+    __device__ explicit Bars(uint32_t base)
+        : q(base), kv_full(base + 8), kv_empty(kv_full + 8 * STAGES), s(kv_empty + 8 * STAGES),
+          p(s + 16), o(p + 16), done(o + 16), clean(done + 8) {}
+};
+
+// Rows [lo, hi) that row i sees; (0, 0) for a row behind the last document.
 // Safe for any content of cu_seqlens.
 __device__ __forceinline__ int2 seen_rows(const Params& p, int i) {
     int d = 0, lo = 0, hi = p.tokens;
@@ -63,61 +120,519 @@ __device__ __forceinline__ int2 seen_rows(const Params& p, int i) {
     return make_int2(lo, hi);
 }
 
-__device__ __forceinline__ float warp_sum(float x) {
+// What every role needs to know of the CTA's work.  Key tile j is rows
+// kv0 + 128 j on; query tile t takes part in the key tiles [first[t], last[t]).
+struct Work {
+    int row0, head, kv0, tiles, first[2], last[2];
+    int clear_lo, clear_hi;            // keys [clear_lo, clear_hi) are seen by every valid row
+    __device__ bool active(int t, int j) const { return j >= first[t] && j < last[t]; }
+    // Whether some row does not see some key of tile j.
+    __device__ bool edge(int j) const {
+        const int k = kv0 + j * TILE;
+        return k < clear_lo || k + TILE > clear_hi;
+    }
+};
+
+// `seen[t]` holds the ranges of tile t's first and last row that belongs to a
+// document; `valid` rows of the CTA do.
+__device__ __forceinline__ Work make_work(const int2 (*seen)[2], int row0, int head, int valid) {
+    Work w;
+    w.row0 = row0;
+    w.head = head;
+    w.kv0 = seen[0][0].x;
+    w.clear_lo = seen[valid > TILE][1].x;
+    w.clear_hi = seen[0][0].y;
+    w.tiles = 0;
+    for (int t = 0; t < 2; ++t) {
+        w.first[t] = w.last[t] = 0;
+        if (valid > t * TILE) {
+            w.first[t] = max(seen[t][0].x - w.kv0, 0) / TILE;
+            w.last[t] = max((seen[t][1].y - w.kv0 + TILE - 1) / TILE, w.first[t]);
+        }
+        w.tiles = max(w.tiles, w.last[t]);
+    }
+    return w;
+}
+
+__device__ __forceinline__ bool drain_wait(uint32_t bar, uint32_t parity, uint64_t timeout_ns,
+                                           int32_t* status) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity)) {
+        if (globaltimer_ns() - t0 > timeout_ns) {
+            report_status(status, FU_DEV_PIPELINE_TIMEOUT, W_DRAIN);
+            return false;
+        }
+    }
+    return true;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], BF16 inputs, FP32 accumulate.
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Each thread's 32 (16) registers -> consecutive columns of its TMEM lane.
+__device__ __forceinline__ void tmem_st_32cols(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+          "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+          "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+          "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+          "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_16cols(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+          "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+          "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16x2_rn(float lo, float hi) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// ------------------------------------------------------------ loads
+// Ring order: K_0, V_0, K_1, V_1, ...
+__device__ void run_loads(const Params& p, const Work& w, uint8_t* smem, const Bars& b,
+                          volatile int* abort_flag) {
+    const uint32_t q = smem_u32(smem + OFF_Q), ring = smem_u32(smem + OFF_KV);
+    const int q_col = w.head * D, kv_col = w.head / p.group * D;
+    mbar_arrive_expect_tx(b.q, 2 * TILE_BYTES);
+    for (int t = 0; t < 2; ++t)
+        for (int c = 0; c < 2; ++c)
+            tma_load_2d(q + t * TILE_BYTES + c * BOX_BYTES, &p.tm_q, b.q, q_col + 64 * c,
+                        w.row0 + t * TILE);
+    int i = 0;
+    for (; i < 2 * w.tiles; ++i) {
+        const int s = i % STAGES, use = i / STAGES;
+        if (!fu_wait_parity(b.kv_empty + 8 * s, (use & 1) ^ 1, abort_flag, p.timeout_ns, p.status,
+                            W_KV_EMPTY))
+            break;
+        mbar_arrive_expect_tx(b.kv_full + 8 * s, TILE_BYTES);
+        for (int c = 0; c < 2; ++c)
+            tma_load_2d(ring + s * TILE_BYTES + c * BOX_BYTES, i & 1 ? &p.tm_v : &p.tm_k,
+                        b.kv_full + 8 * s, kv_col + 64 * c, w.kv0 + (i >> 1) * TILE);
+    }
+    // What was issued must land before shared memory is released, whatever the
+    // other roles did.
+    drain_wait(b.q, 0, p.timeout_ns, p.status);
+    for (int k = i > STAGES ? i - STAGES : 0; k < i; ++k)
+        drain_wait(b.kv_full + 8 * (k % STAGES), (k / STAGES) & 1, p.timeout_ns, p.status);
+}
+
+// ------------------------------------------------------------ MMA
+__device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t tmem, const Bars& b,
+                        volatile int* abort_flag) {
+    // S = Q K^T: both K-major.  O += P V: P from TMEM, V [keys, dims] MN-major.
+    const uint32_t idesc_s = make_idesc_bf16_f32(TILE, TILE, false, false) | (p.negate << 13);
+    constexpr uint32_t idesc_o = make_idesc_bf16_f32(TILE, D, false, true);
+    const uint32_t q = smem_u32(smem + OFF_Q), ring = smem_u32(smem + OFF_KV);
+    const auto wait = [&](uint32_t bar, uint32_t parity, int where) {
+        return fu_wait_parity(bar, parity, abort_flag, p.timeout_ns, p.status, where);
+    };
+    uint32_t p_phase[2] = {0, 0};
+    bool ok = wait(b.q, 0, W_Q);
+    // Step j: the products P V of key tile j, each followed by the same query
+    // tile's scores of key tile j + 1.
+    for (int j = -1; ok && j < w.tiles; ++j) {
+        const int iv = 2 * j + 1, ik = 2 * j + 2;       // ring positions of V_j and K_(j+1)
+        const int sv = iv % STAGES, sk = ik % STAGES;
+        if (j >= 0) {
+            if (w.edge(j)) {
+                ok = wait(b.clean + 8 * (j % STAGES), (j / STAGES) & 1, W_CLEAN);
+            } else {
+                ok = wait(b.kv_full + 8 * sv, (iv / STAGES) & 1, W_KV_FULL);
+            }
+            if (!ok) break;
+        }
+        if (j + 1 < w.tiles && !(ok = wait(b.kv_full + 8 * sk, (ik / STAGES) & 1, W_KV_FULL))) break;
+        tc_fence_after();
+        for (int t = 0; t < 2; ++t) {
+            if (j >= 0 && w.active(t, j)) {
+                if (!(ok = wait(b.p + 8 * t, p_phase[t], W_P))) break;
+                p_phase[t] ^= 1;
+                tc_fence_after();
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    return x;
+                for (int k = 0; k < TILE / 16; ++k)
+                    tc_mma_bf16_ts(tmem + TM_O + t * TILE, tmem + TM_S + t * TILE + 8 * k,
+                                   make_smem_desc_sw128(ring + sv * TILE_BYTES + k * 16 * 128,
+                                                        BOX_BYTES, 1024),
+                                   idesc_o, j > w.first[t] || k > 0);
+                if (j + 1 == w.last[t]) tc_commit(b.o + 8 * t);
+            }
+            if (j >= 0 && t == 1) tc_commit(b.kv_empty + 8 * sv);
+            if (w.active(t, j + 1)) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = (k / 4) * BOX_BYTES + (k % 4) * 32;
+                    tc_mma_bf16(tmem + TM_S + t * TILE,
+                                make_smem_desc_sw128(q + t * TILE_BYTES + at, 16, 1024),
+                                make_smem_desc_sw128(ring + sk * TILE_BYTES + at, 16, 1024),
+                                idesc_s, k > 0);
+                }
+                tc_commit(b.s + 8 * t);
+            }
+            if (j + 1 < w.tiles && t == 1) tc_commit(b.kv_empty + 8 * sk);
+        }
+    }
+    // Every MMA this thread issued must finish before TMEM is released.
+    tc_commit(b.done);
+    drain_wait(b.done, 0, p.timeout_ns, p.status);
 }
 
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-    const uint2 r = *reinterpret_cast<const uint2*>(p);
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.x));
-    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.y));
-    return make_float4(a.x, a.y, b.x, b.y);
+// ------------------------------------------------------------ V at a mask's edge
+// Every V tile is counted (on a ring of barriers of its own), so that neither
+// side gets more than the ring ahead; only those at an edge are looked at.
+__device__ void run_clean(const Params& p, const Work& w, uint8_t* smem, const Bars& b,
+                          volatile int* abort_flag, volatile int* found) {
+    const int me = threadIdx.x & 63;
+    for (int j = 0; j < w.tiles; ++j) {
+        const int i = 2 * j + 1, s = i % STAGES;
+        if (!fu_wait_parity(b.kv_full + 8 * s, (i / STAGES) & 1, abort_flag, p.timeout_ns, p.status,
+                            W_KV_FULL))
+            return;
+        uint4* v = reinterpret_cast<uint4*>(smem + OFF_KV + s * TILE_BYTES);
+        bool wrote = false;
+#pragma unroll 8
+        for (int o = me; o < (w.edge(j) ? TILE_BYTES / 16 : 0); o += 64) {
+            uint4 x = v[o];
+            uint32_t* word = &x.x;
+            bool odd = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // A BF16 is not finite if its exponent bits are all set.
+                const uint32_t bad = __vcmpeq2(word[k] & 0x7f807f80u, 0x7f807f80u);
+                word[k] &= ~bad;
+                odd = odd || bad != 0;
+            }
+            if (odd) {
+                v[o] = x;
+                wrote = true;
+            }
+        }
+        if (wrote) {
+            *found = 1;
+            fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if ((me & 31) == 0) mbar_arrive(b.clean + 8 * (j % STAGES));
+    }
 }
 
-__global__ void __launch_bounds__(32 * WARPS) attention_kernel(const Params p) {
+// ------------------------------------------------------------ softmax
+// kMode: 1 scores capped by a tanh, 2 lowered with distance (3 both).
+template <int kMode>
+__device__ void run_softmax(const Params& p, const Work& w, uint8_t* smem, uint32_t tmem,
+                            const Bars& b, int t, int2 seen, bool valid,
+                            volatile int* abort_flag, volatile int* found) {
+    const int lane = threadIdx.x & 31;
+    const int warp = (threadIdx.x >> 5) & 3;              // of this tile
+    const int row = w.row0 + t * TILE + warp * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const uint32_t tm_s = tmem + TM_S + t * TILE + lanes, tm_o = tmem + TM_O + t * TILE + lanes;
+    // Scores in units of log2: x = c * s here, m in the units of s (so c m is
+    // its logarithm), or with a cap or a bias x = s, c = 1.
+    const float c = kMode ? 1.f : fmaxf(p.scale * LOG2E, 1e-30f);
+    const float slope =
+        kMode & 2 ? __ldg(p.alibi_slopes + w.head) * LOG2E : 0.f;
+    // tanh(z) = 1 - 2 / (1 + 2^(2 log2(e) z)): its error is absolute, 2^-22 of
+    // the cap, which is what a score needs.
+    const float cap_in = kMode & 1 ? 2.f * LOG2E * p.scale / p.softcap : 0.f;
+    const float cap_out = kMode & 1 ? p.softcap * LOG2E : 0.f;
+    const float lin = p.scale * LOG2E;
+    // A row without a document is computed like one that sees everything, and
+    // not stored.
+    const int lo = valid ? seen.x : INT_MIN / 2, hi = valid ? seen.y : INT_MAX / 2;
+
+    float m = -INFINITY, l = 0.f;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int j = w.first[t]; j < w.last[t]; ++j) {
+        ok = fu_wait_parity(b.s + 8 * t, phase, abort_flag, p.timeout_ns, p.status, W_S);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        phase ^= 1;
+        tc_fence_after();
+        uint32_t r[TILE];
+        float* s = reinterpret_cast<float*>(r);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            tmem_ld_32cols(tm_s + 32 * k, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * k));
+        tmem_ld_wait();
+        const int k0 = w.kv0 + j * TILE;
+        if (kMode) {
+            const float at = static_cast<float>(row - k0);
+#pragma unroll
+            for (int k = 0; k < TILE; ++k) {
+                float x = s[k];
+                if (kMode & 1) {
+                    const float e = ex2(x * cap_in);
+                    x = fmaf(-2.f * cap_out, __fdividef(1.f, 1.f + e), cap_out);
+                } else {
+                    x *= lin;
+                }
+                if (kMode & 2) x = fmaf(-slope, fabsf(at - static_cast<float>(k)), x);
+                s[k] = x;
+            }
+        }
+        const int from = lo - k0, to = hi - k0;
+        if (__any_sync(0xffffffffu, from > 0 || to < TILE)) {
+#pragma unroll
+            for (int k = 0; k < TILE; ++k)
+                s[k] = k >= from && k < to ? s[k] : -INFINITY;
+        }
+        float best[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int k = 4; k < TILE; k += 4)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) best[q] = fmaxf(best[q], s[k + q]);
+        const float top = fmaxf(m, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])));
+        if (j == w.first[t]) {
+            m = top;
+        } else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
+            const float f = top == -INFINITY ? 1.f : ex2((m - top) * c);
+            l *= f;
+            m = top;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t o[32];
+                tmem_ld_32cols(tm_o + 32 * k, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+                tmem_st_32cols(tm_o + 32 * k, o);
+            }
+        }
+        const float base = m == -INFINITY ? 0.f : m * c;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const float x = ex2(fmaf(s[32 * k + 2 * q], c, -base));
+                const float y = ex2(fmaf(s[32 * k + 2 * q + 1], c, -base));
+                sum[(2 * q) & 3] += x;
+                sum[(2 * q + 1) & 3] += y;
+                packed[q] = pack_bf16x2_rn(x, y);
+            }
+            tmem_st_16cols(tm_s + 16 * k, packed);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b.p + 8 * t);
+    }
+    if (w.first[t] == w.last[t] || !ok) return;
+
+    // out = O / l, through this tile's Q rows in shared memory (no longer
+    // needed): a thread writes its row, then the warp's 32 rows leave as whole
+    // 256-byte rows.
+    ok = fu_wait_parity(b.o + 8 * t, 0, abort_flag, p.timeout_ns, p.status, W_O);
+    if (!__all_sync(0xffffffffu, ok)) return;
+    tc_fence_after();
+    const float inv = 1.f / l;
+    const bool poison = *found != 0;
+    uint8_t* stage = smem + OFF_Q + t * TILE_BYTES + warp * 32 * 256;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+        uint32_t o[32];
+        tmem_ld_32cols(tm_o + 32 * k, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * inv);
+        if (poison && valid) {
+            // What run_clean() took out, for the rows that see it.
+            for (int j = w.first[t]; j < w.last[t]; ++j) {
+                if (!w.edge(j)) continue;
+                const int a = max(lo, w.kv0 + j * TILE), e = min(hi, w.kv0 + (j + 1) * TILE);
+                for (int key = a; key < e; ++key) {
+                    const __nv_bfloat16* v = p.v + key * p.v_stride + w.head / p.group * D + 32 * k;
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) {
+                        const float x = __bfloat162float(v[q]);
+                        if (!isfinite(x)) o[q] = __float_as_uint(__uint_as_float(o[q]) + x);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int chunk = 4 * k + q;
+            const uint32_t* x = o + 8 * q;
+            *reinterpret_cast<uint4*>(stage + lane * 256 + ((chunk ^ (lane & 7)) << 4)) = make_uint4(
+                pack_bf16x2_rn(__uint_as_float(x[0]), __uint_as_float(x[1])),
+                pack_bf16x2_rn(__uint_as_float(x[2]), __uint_as_float(x[3])),
+                pack_bf16x2_rn(__uint_as_float(x[4]), __uint_as_float(x[5])),
+                pack_bf16x2_rn(__uint_as_float(x[6]), __uint_as_float(x[7])));
+        }
+    }
+    const uint32_t stored = __ballot_sync(0xffffffffu, valid);
+    __syncwarp();
+    __nv_bfloat16* dst = p.out + static_cast<int64_t>(row - lane) * p.out_stride + w.head * D;
+#pragma unroll 4
+    for (int r = lane >> 4; r < 32; r += 2) {
+        const int chunk = lane & 15;
+        if (stored >> r & 1)
+            *reinterpret_cast<uint4*>(dst + r * p.out_stride + 8 * chunk) =
+                *reinterpret_cast<const uint4*>(stage + r * 256 + ((chunk ^ (r & 7)) << 4));
+    }
+}
+
+// ------------------------------------------------------------ kernel
+template <int kMode>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+attention_kernel(const __grid_constant__ Params p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int warp = threadIdx.x >> 5;
+    const Bars b(smem_u32(smem + OFF_BAR));
+    int2 (*seen)[2] = reinterpret_cast<int2 (*)[2]>(smem + OFF_SEEN);
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
+    volatile int* found = reinterpret_cast<volatile int*>(smem + OFF_MISC + 8);
+
+    // Prologue: shared memory, TMEM and parameters only (it may overlap the
+    // previous kernel of the stream under a programmatic dependent launch).
+    if (threadIdx.x == 0) {
+        mbar_init(b.q, 1);
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(b.kv_full + 8 * s, 1);
+            mbar_init(b.kv_empty + 8 * s, 1);
+            mbar_init(b.clean + 8 * s, 2);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(b.s + 8 * t, 1);
+            mbar_init(b.p + 8 * t, 4);
+            mbar_init(b.o + 8 * t, 1);
+        }
+        mbar_init(b.done, 1);
+        *abort_flag = 0;
+        *found = 0;
+        fence_mbar_init();
+        tma_prefetch_desc(&p.tm_q);
+        tma_prefetch_desc(&p.tm_k);
+        tma_prefetch_desc(&p.tm_v);
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(tmem_holder), TMEM_COLS);
+        tmem_relinquish();
+    }
+    // Global memory from here on: the previous kernel of the stream is done.
     grid_dependency_wait();
     grid_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && p.cu_seqlens != nullptr) {
-        for (int d = threadIdx.x; d <= p.docs; d += blockDim.x) {
-            const int c = p.cu_seqlens[d];
-            const int before = d > 0 ? p.cu_seqlens[d - 1] : 0;
-            if (c < before || c > p.tokens || (d == 0 && c != 0))
+
+    // The longest rows first: with a causal mask the last CTAs to start then
+    // have the least to do.
+    const int head = blockIdx.x % p.q_heads;
+    const int row0 = (gridDim.x / p.q_heads - 1 - blockIdx.x / p.q_heads) * ROWS;
+    if (blockIdx.x == 0 && p.cu_seqlens != nullptr) {
+        for (int d = threadIdx.x; d <= p.docs; d += NUM_THREADS) {
+            const int x = __ldg(p.cu_seqlens + d);
+            const int before = d > 0 ? __ldg(p.cu_seqlens + d - 1) : 0;
+            if (x < before || x > p.tokens || (d == 0 && x != 0))
                 report_status(p.status, FU_DEV_LENGTHS, W_CU_SEQLENS);
         }
     }
-    const int i = blockIdx.x * WARPS + (threadIdx.x >> 5);
-    const int h = blockIdx.y;
-    if (i >= p.tokens) return;
-    const int2 seen = seen_rows(p, i);
-    if (seen.x >= seen.y) return;
-    const int hk = h / p.group;
-    const float4 q = load4(p.q + i * p.q_stride + h * D + 4 * lane);
-    const float slope = p.alibi_slopes != nullptr ? p.alibi_slopes[h] : 0.f;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = seen.x; j < seen.y; ++j) {
-        const float4 k = load4(p.k + j * p.k_stride + hk * D + 4 * lane);
-        const float4 v = load4(p.v + j * p.v_stride + hk * D + 4 * lane);
-        float x = p.scale * warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w);
-        if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-        x -= slope * fabsf(static_cast<float>(i - j));
-        const float m2 = fmaxf(m, x);
-        const float old = m == m2 ? 1.f : __expf(m - m2);
-        const float w = __expf(x - m2);
-        m = m2;
-        l = l * old + w;
-        o.x = o.x * old + w * v.x;
-        o.y = o.y * old + w * v.y;
-        o.z = o.z * old + w * v.z;
-        o.w = o.w * old + w * v.w;
+    int rows = p.tokens;                               // rows of documents
+    if (p.cu_seqlens != nullptr) rows = min(max(__ldg(p.cu_seqlens + p.docs), 0), p.tokens);
+    const int valid = min(rows - row0, ROWS);
+    int2 mine = make_int2(0, 0);
+    if (warp < 8) {
+        const int i = threadIdx.x, t = i / TILE;
+        if (row0 + i < p.tokens) mine = seen_rows(p, row0 + i);
+        if (i == t * TILE) seen[t][0] = mine;
+        if (i == min(valid, (t + 1) * TILE) - 1) seen[t][1] = mine;
     }
-    __nv_bfloat162 r[2] = {__floats2bfloat162_rn(o.x / l, o.y / l),
-                           __floats2bfloat162_rn(o.z / l, o.w / l)};
-    *reinterpret_cast<uint2*>(p.out + i * p.out_stride + h * D + 4 * lane) =
-        *reinterpret_cast<const uint2*>(r);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    if (valid > 0) {
+        const Work w = make_work(seen, row0, head, valid);
+        if (warp < 8) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+            run_softmax<kMode>(p, w, smem, tmem, b, warp >> 2, mine, mine.x < mine.y, abort_flag,
+                               found);
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+            if (warp == 8) {
+                if ((threadIdx.x & 31) == 0) run_loads(p, w, smem, b, abort_flag);
+            } else if (warp == 9) {
+                if ((threadIdx.x & 31) == 0) run_mma(p, w, smem, tmem, b, abort_flag);
+            } else {
+                run_clean(p, w, smem, b, abort_flag, found);
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// ------------------------------------------------------------ host side
+// BF16 [rows, cols] with a row stride, box {64, 128}, 128-byte swizzle.
+static int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t cols,
+                       int64_t stride, const char* what) {
+    auto fn = encode_tiled_fn();
+    if (fn == nullptr) return set_error(FU_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+    const cuuint32_t box[2] = {64, TILE};
+    const cuuint32_t elem[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+                    strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return set_error(FU_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with %d", what,
+                         static_cast<int>(r));
+    return FU_OK;
+}
+
+typedef void (*Kernel)(const Params);
+
+// Raises the kernels' shared-memory limit once per device.
+static cudaError_t prepare(int device) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    for (Kernel k : {attention_kernel<0>, attention_kernel<1>, attention_kernel<2>,
+                     attention_kernel<3>}) {
+        cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             SMEM_ALLOC);
+        if (e != cudaSuccess) return e;
+    }
+    if (device < 64) done.fetch_or(bit, std::memory_order_release);
+    return cudaSuccess;
 }
 
 }  // namespace attention
@@ -155,31 +670,50 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
         return set_error(FU_ERR_DEVICE, "an earlier launch reported device status 0x%x",
                          static_cast<unsigned>(*a->status_host));
 
+    const int64_t blocks = (a->tokens + attention::ROWS - 1) / attention::ROWS * a->q_heads;
+    if (blocks > INT32_MAX)
+        return set_error(FU_ERR_INVALID, "tokens * q_heads is too large for one call");
+
     attention::Params p = {};
-    p.q = static_cast<const __nv_bfloat16*>(a->q);
-    p.k = static_cast<const __nv_bfloat16*>(a->k);
+    int rc = attention::encode_rows(&p.tm_q, a->q, a->tokens, a->q_heads * attention::D,
+                                    a->q_stride, "q");
+    if (rc == FU_OK)
+        rc = attention::encode_rows(&p.tm_k, a->k, a->tokens, a->kv_heads * attention::D,
+                                    a->k_stride, "k");
+    if (rc == FU_OK)
+        rc = attention::encode_rows(&p.tm_v, a->v, a->tokens, a->kv_heads * attention::D,
+                                    a->v_stride, "v");
+    if (rc != FU_OK) return rc;
     p.v = static_cast<const __nv_bfloat16*>(a->v);
     p.out = static_cast<__nv_bfloat16*>(a->out);
-    p.q_stride = a->q_stride;
-    p.k_stride = a->k_stride;
     p.v_stride = a->v_stride;
     p.out_stride = a->out_stride;
     p.cu_seqlens = a->cu_seqlens;
     p.prefix_lens = a->prefix_lens;
     p.alibi_slopes = a->alibi_slopes;
     p.status = a->status;
+    p.timeout_ns = a->timeout_ns ? a->timeout_ns : FU_DEFAULT_TIMEOUT_NS;
     p.tokens = static_cast<int32_t>(a->tokens);
     p.docs = a->docs;
+    p.q_heads = a->q_heads;
     p.group = a->q_heads / a->kv_heads;
     p.causal = a->causal;
-    p.scale = a->scale;
+    p.negate = a->scale < 0.f ? 1u : 0u;
+    p.scale = std::fabs(a->scale);
     p.softcap = a->softcap;
 
     DeviceGuard guard(a->device);
     if (!guard.ok()) return set_error(FU_ERR_INVALID, "device %d is not available", a->device);
-    Launch launch(dim3((p.tokens + attention::WARPS - 1) / attention::WARPS, a->q_heads),
-                  dim3(32 * attention::WARPS), 0, stream, (flags & FU_FWD_NO_PDL) == 0);
-    cudaError_t e = cudaLaunchKernelEx(&launch.cfg, attention::attention_kernel, p);
+    cudaError_t e = attention::prepare(a->device);
+    if (e == cudaSuccess) {
+        const attention::Kernel kernels[4] = {
+            attention::attention_kernel<0>, attention::attention_kernel<1>,
+            attention::attention_kernel<2>, attention::attention_kernel<3>};
+        const int mode = (a->softcap > 0.f ? 1 : 0) | (a->alibi_slopes != nullptr ? 2 : 0);
+        Launch launch(dim3(static_cast<unsigned>(blocks)), dim3(attention::NUM_THREADS),
+                      attention::SMEM_ALLOC, stream, (flags & FU_FWD_NO_PDL) == 0);
+        e = cudaLaunchKernelEx(&launch.cfg, kernels[mode], p);
+    }
     if (e != cudaSuccess) return set_error(FU_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return FU_OK;
 }
