@@ -2,9 +2,12 @@
 // tokens, and the attention of single tokens that reads them.
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -230,10 +233,49 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 }
 
 // ------------------------------------------------------------ attention
+// Decode: per (sequence, K/V head) the group's query heads are the rows of a
+// small matrix product over the sequence's blocks of 64 tokens.  One pass over
+// the cache bounds it (256 bytes per token and head), so the work is split
+// along the tokens over all SMs and joined afterwards:
+//
+//   attention_split_kernel   CTAs of 4 warps; a warp takes whole blocks, with
+//                            an online softmax of its own; the CTA joins its
+//                            warps and writes either the output or a partial
+//   attention_join_kernel    joins the partials of split (sequence, head)s,
+//                            in their order, so results do not depend on timing
+//
+// A block is two contiguous 8 KiB tiles (K, V transposed), which each warp has
+// copied into a ring of its own in shared memory (cp.async.bulk), across the
+// borders of sequences.  From there mma.sync (m16n8k16, f16, FP32 accumulation)
+// reads its operands as they lie, 16 bytes per lane and load, with nothing
+// shuffled:
+//   * e4m3 becomes f16 exactly.  The order of a product's summation index is
+//     free as long as both operands agree, so lane (g, t) = (lane / 4, lane % 4)
+//     takes 16 consecutive dims of a K row, and the matching dims of q.
+//   * Scores come out as rows = query heads, columns = tokens; with K row
+//     16 (n / 2) + 2 j + n % 2 as column n of score tile j, lane (g, t) ends up
+//     with row g's scores of tokens 16 t .. 16 t + 15, and these are what the
+//     second product needs from it next to 16 bytes of a row of V transposed.
+//   * q is scaled by a power of two per row, so that f16 holds it; weights are
+//     f16 in [0, 1]; block scales are applied in FP32.
+// tcgen05 would pad 4 to 16 rows to 128; here the tensor work is far below the
+// time of the loads.
+//
+// The unfinished block is BF16 and takes the same route with BF16 products, its
+// weights as a sum of two BF16 so that they keep 16 bits.
+constexpr int WARPS = 4;
+constexpr int SPLIT_THREADS = 32 * WARPS;
+constexpr int MAX_BATCH = 512;         // sequences per launch (their prefix sums sit in shared memory)
+constexpr int TILE_BYTES = BLOCK * D;  // one stage of a warp's ring: K or V of a block
+constexpr float LOG2E = 1.4426950408889634f;
+
 struct AttentionParams {
-    const uint8_t* blocks[2];
-    const float* scales[2];
-    const __nv_bfloat16* tail[2];
+    const uint8_t* k_blocks;
+    const uint8_t* v_blocks;
+    const float* k_scales;
+    const float* v_scales;
+    const __nv_bfloat16* k_tail;
+    const __nv_bfloat16* v_tail;
     const int32_t* block_table;
     const __nv_bfloat16* q;
     __nv_bfloat16* out;
@@ -242,75 +284,744 @@ struct AttentionParams {
     const int32_t* seq_lens;
     const float* alibi_slopes;
     int32_t* status;
-    int32_t kv_heads, num_blocks, max_seqs, max_blocks, seqs, group;
+    struct Plan* plan;
+    float* partial;                    // [CTA][2][rows of a unit][PART]
+    int32_t kv_heads, num_blocks, max_seqs, max_blocks, seqs, group, row_tiles, ctas;
     float scale, softcap;
 };
+constexpr int PART = D + 4;            // one row of a partial: 128 sums, m, l, padding
 
-__device__ __forceinline__ float warp_sum(float x) {
+// How the call's blocks are dealt to the CTAs.  The items are the blocks of
+// all (sequence, K/V head, row tile)s -- pairs -- one after another; sequence
+// i's begin at first[i], nb blocks for each of its pairs.
+//   aligned (few pairs): a CTA takes up to `share` blocks of one pair; the
+//     units of sequence i begin at unit[i] = sum of ceil(nb / share) * pairs.
+//   otherwise a CTA takes `share` consecutive items, of as many pairs as that is.
+struct alignas(16) Plan {
+    int32_t items, share, aligned, pad;
+    int32_t first[MAX_BATCH + 1];
+    int32_t unit[MAX_BATCH + 1];
+};
+
+static_assert(sizeof(Plan) % 16 == 0, "the partials behind it are written 16 bytes at a time");
+
+// Shared memory of a split CTA.  Three stages a warp put 192 KiB per SM in
+// flight; the wide rows' joining area leaves room for two.
+template <bool kWide>
+struct SplitSmem {
+    static constexpr int STAGES = kWide ? 2 : 3, ROWS = kWide ? 16 : 8;
+    uint8_t ring[WARPS][STAGES][TILE_BYTES];
+    float o[WARPS - 1][ROWS][PART];
+    uint64_t full[WARPS][STAGES];
+    int32_t first[MAX_BATCH + 1];
+    int32_t unit[MAX_BATCH / 4 + 1];
+    int32_t scan[WARPS];
+};
+static_assert(2 * (sizeof(SplitSmem<false>) + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (sizeof(SplitSmem<true>) + 1024) <= 228 * 1024, "two CTAs per SM");
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two e4m3 bytes (the low or high half of w) -> two f16.
+template <int kHalf>
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, %2;\n\t}" : "=r"(r) : "r"(w), "h"(static_cast<uint16_t>(w >> (16 * kHalf))));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// `bytes` (a multiple of 16) of global memory -> shared memory, counted on `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes "
+                 "[%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// A warp's running softmax and output for its rows: row g (and g + 8 if kWide).
+// o[h][dn][c] is row g + 8 h, dim 32 t + 16 c + dn of lane (g, t).
+template <bool kWide>
+struct Rows {
+    static constexpr int H = kWide ? 2 : 1;
+    float m[H], l[H], o[H][16][2];
+    __device__ void clear() {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    return x;
+        for (int h = 0; h < H; ++h) {
+            m[h] = -INFINITY;
+            l[h] = 0.f;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) o[h][d][0] = o[h][d][1] = 0.f;
+        }
+    }
+};
+
+// The score's path from the raw product to log2 units, and what it needs of a row.
+template <int kMode>
+struct Score {
+    float factor, cap_out, slope;      // per row; with a cap `factor` is that of 2 log2(e) z
+    __device__ float operator()(float raw, float block_scale, int distance) const {
+        float x = raw * (factor * block_scale);
+        if (kMode & 1) {
+            // cap tanh(z) = cap (1 - 2 / (1 + 2^(2 log2(e) z))): an absolute error of 2^-22 cap.
+            x = fmaf(-2.f * cap_out, __fdividef(1.f, 1.f + ex2(x)), cap_out);
+        }
+        if (kMode & 2) x = fmaf(-slope, static_cast<float>(distance), x);
+        return x;
+    }
+};
+
+// One block's scores s[h][j][c] (token 16 t + 2 j + c of the block, already in
+// log2 units, -inf where not seen) -> weights in place; returns the factor of
+// what was summed before.
+template <bool kWide>
+__device__ __forceinline__ void softmax_step(Rows<kWide>& r, float (&s)[Rows<kWide>::H][8][2],
+                                             float (&old)[Rows<kWide>::H]) {
+#pragma unroll
+    for (int h = 0; h < Rows<kWide>::H; ++h) {
+        float top = r.m[h];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fmaxf(s[h][j][0], s[h][j][1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float base = top == -INFINITY ? 0.f : top;
+        old[h] = ex2(r.m[h] - base);
+        r.m[h] = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                s[h][j][c] = ex2(s[h][j][c] - base);
+                sum += s[h][j][c];
+            }
+        r.l[h] = fmaf(r.l[h], old[h], sum);            // this lane's tokens only
+    }
 }
 
-__device__ __forceinline__ float e4m3(uint8_t x) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3)));
-}
+// A warp's way through its CTA's items [at, end): pair by pair, within a pair
+// every WARPS-th block.  The feed of the ring and the arithmetic each have one.
+struct Walk {
+    int at, end;                       // items of the CTA not entered yet
+    int i, pair, b0, b1, nb;           // the current pair, its blocks here [b0, b1) of nb
+    int slot, len, b;                  // b: the warp's current block
+    int id;                            // lane k: cache block of the warp's k-th of 32 blocks
 
-// One warp per (sequence, query head); lane l holds dims 4l..4l+3.
-__global__ void __launch_bounds__(32) attention_kernel(const AttentionParams p) {
+    __device__ bool enter(const AttentionParams& p, const int32_t* first, int pairs, int warp) {
+        if (at >= end) return false;
+        i = 0;                         // the last sequence that begins at `at` or before
+        for (int hi = p.seqs; hi - i > 1;) {
+            const int mid = (i + hi) >> 1;
+            if (first[mid] <= at) i = mid; else hi = mid;
+        }
+        nb = (first[i + 1] - first[i]) / pairs;
+        pair = (at - first[i]) / nb;
+        b0 = at - first[i] - pair * nb;
+        b1 = min(nb, b0 + end - at);
+        at += b1 - b0;
+        slot = __ldg(p.slots + i);
+        len = __ldg(p.seq_lens + i);
+        b = b0 + warp;
+        return true;
+    }
+    __device__ bool is_full() const { return b < len / BLOCK; }
+    // Cache block of block b (a full one), -1 if it is outside the cache.  The
+    // warp looks up 32 at a time; `fresh` says that it just did.
+    __device__ int lookup(const AttentionParams& p, int warp, int lane, bool& fresh) {
+        const int k = (b - b0 - warp) / WARPS & 31;
+        fresh = k == 0;
+        if (fresh) {
+            const int mine = b + WARPS * lane;
+            id = mine < min(b1, len / BLOCK)
+                     ? __ldg(p.block_table + static_cast<int64_t>(slot) * p.max_blocks + mine) : 0;
+            if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.num_blocks)) id = -1;
+        }
+        return __shfl_sync(0xffffffffu, id, k);
+    }
+};
+
+template <bool kWide, int kMode>
+__global__ void __launch_bounds__(SPLIT_THREADS, 2)
+attention_split_kernel(const AttentionParams p) {
+    using Smem = SplitSmem<kWide>;
+    constexpr int H = Rows<kWide>::H, ROWS = 8 * H, STAGES = Smem::STAGES;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&sm.full[warp][s]), 1);
+        fence_mbar_init();
+    }
     grid_dependency_wait();
     grid_launch_dependents();
-    const int i = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-    const int h = head / p.group;
-    const int slot = p.slots[i], len = p.seq_lens[i];
-    if (slot < 0) return;
-    if (slot >= p.max_seqs || len < 0 || len > p.max_blocks * BLOCK) {
-        if (lane == 0)
-            report_status(p.status, slot >= p.max_seqs ? FU_DEV_CACHE_RANGE : FU_DEV_LENGTHS,
-                          W_ATTENTION);
-        return;
-    }
-    float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int d = 0; d < 4; ++d)
-        q[d] = __bfloat162float(p.q[i * p.q_stride + head * D + 4 * lane + d]);
-    const float slope = p.alibi_slopes != nullptr ? p.alibi_slopes[head] : 0.f;
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < len; ++j) {
-        const int b = j / BLOCK, r = j % BLOCK;
-        float k[4], v[4];
-        if (b < len / BLOCK) {
-            const int id = p.block_table[static_cast<int64_t>(slot) * p.max_blocks + b];
-            if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.num_blocks)) {
-                if (lane == 0) report_status(p.status, FU_DEV_CACHE_RANGE, W_ATTENTION);
-                continue;
-            }
-            const int64_t at = static_cast<int64_t>(id) * p.kv_heads + h;
-            for (int d = 0; d < 4; ++d) {
-                k[d] = e4m3(p.blocks[0][at * BLOCK * D + r * D + 4 * lane + d]) * p.scales[0][at];
-                v[d] = e4m3(p.blocks[1][at * BLOCK * D + (4 * lane + d) * BLOCK + r]) *
-                       p.scales[1][at];
-            }
-        } else {
-            const int64_t at =
-                ((static_cast<int64_t>(slot) * p.kv_heads + h) * BLOCK + r) * D + 4 * lane;
-            for (int d = 0; d < 4; ++d) {
-                k[d] = __bfloat162float(p.tail[0][at + d]);
-                v[d] = __bfloat162float(p.tail[1][at + d]);
+
+    // Prefix sums of the sequences' blocks; a row that is padding or does not
+    // fit has none.
+    const int pairs = p.kv_heads * p.row_tiles;
+    int total = 0;
+    for (int i0 = 0; i0 < p.seqs; i0 += SPLIT_THREADS) {
+        const int i = i0 + threadIdx.x;
+        int nb = 0;
+        if (i < p.seqs) {
+            const int slot = __ldg(p.slots + i), len = __ldg(p.seq_lens + i);
+            if (slot >= 0) {
+                if (slot >= p.max_seqs || len < 0 || len > p.max_blocks * BLOCK) {
+                    if (blockIdx.x == 0)
+                        report_status(p.status,
+                                      slot >= p.max_seqs ? FU_DEV_CACHE_RANGE : FU_DEV_LENGTHS,
+                                      W_ATTENTION);
+                } else {
+                    nb = (len + BLOCK - 1) / BLOCK;
+                    // A sequence without tokens: its output is 0, and nobody else writes it.
+                    if (len == 0 && i % gridDim.x == blockIdx.x)
+                        for (int c = 0; c < p.kv_heads * p.group * D; c += 8)
+                            *reinterpret_cast<uint4*>(p.out + i * p.out_stride + c) =
+                                make_uint4(0, 0, 0, 0);
+                }
             }
         }
-        float x = p.scale * warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-        if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
-        x -= slope * static_cast<float>(len - 1 - j);
-        const float m2 = fmaxf(m, x);
-        const float old = m == m2 ? 1.f : __expf(m - m2);
-        const float w = __expf(x - m2);
-        m = m2;
-        l = l * old + w;
-        for (int d = 0; d < 4; ++d) o[d] = o[d] * old + w * v[d];
+        int sum = nb;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        if (lane == 31) sm.scan[warp] = sum;
+        __syncthreads();
+        int before = total;
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) before += sm.scan[w];
+            total += sm.scan[w];
+        }
+        if (i < p.seqs) sm.first[i] = (before + sum - nb) * pairs;
+        __syncthreads();
     }
-    for (int d = 0; d < 4; ++d)
-        p.out[i * p.out_stride + head * D + 4 * lane + d] =
-            __float2bfloat16_rn(l == 0.f ? 0.f : o[d] / l);
+    const int items = total * pairs;
+    if (threadIdx.x == 0) sm.first[p.seqs] = items;
+    // Few pairs: each is cut into shares of its own, a multiple of WARPS blocks,
+    // that give at most one to every CTA; else the items are dealt evenly.
+    const int all_pairs = p.seqs * pairs;
+    const bool aligned = all_pairs <= p.ctas / 4;
+    const int over = aligned ? p.ctas - all_pairs : p.ctas;
+    const int each = items / over + (items % over != 0);
+    const int share = max((each + WARPS - 1) / WARPS * WARPS, WARPS);
+    __syncthreads();
+    if (aligned && threadIdx.x == 0) {
+        int units = 0;
+        for (int i = 0; i < p.seqs; ++i) {
+            sm.unit[i] = units;
+            const int nb = (sm.first[i + 1] - sm.first[i]) / pairs;
+            units += (nb + share - 1) / share * pairs;
+        }
+        sm.unit[p.seqs] = units;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i <= p.seqs; i += SPLIT_THREADS) {
+            p.plan->first[i] = sm.first[i];
+            if (aligned) p.plan->unit[i] = sm.unit[i];
+        }
+        if (threadIdx.x == 0) {
+            p.plan->items = items;
+            p.plan->share = share;
+            p.plan->aligned = aligned;
+        }
+    }
+
+    // This CTA's items [at, end), pair by pair.
+    Walk walk = {};
+    if (aligned) {
+        const int u = blockIdx.x;
+        if (u >= sm.unit[p.seqs]) return;
+        int i = 0;
+        while (sm.unit[i + 1] <= u) ++i;
+        const int nb = (sm.first[i + 1] - sm.first[i]) / pairs;
+        const int per = (nb + share - 1) / share;
+        const int pair = (u - sm.unit[i]) / per, part = (u - sm.unit[i]) % per;
+        walk.at = sm.first[i] + pair * nb + part * share;
+        walk.end = min(walk.at + share, sm.first[i] + (pair + 1) * nb);
+    } else {
+        walk.at = min(static_cast<int64_t>(blockIdx.x) * share, static_cast<int64_t>(items));
+        walk.end = min(walk.at + static_cast<int64_t>(share), static_cast<int64_t>(items));
+    }
+    const int begin = walk.at;
+
+    // The feed: each call requests one stage, in the order in which the warp
+    // will read them: K and V of a block; of the unfinished block the 32-row
+    // halves of K, then of V.
+    Walk feed = walk;
+    bool feeding = false;
+    int sub = 0, fed = 0;              // part of the current block; stages requested so far
+    const auto request = [&]() {
+        while (true) {
+            if (!feeding && !feed.enter(p, sm.first, pairs, warp)) return;
+            feeding = true;
+            if (feed.b >= feed.b1) {
+                feeding = false;
+                continue;
+            }
+            const int head = feed.pair / p.row_tiles;
+            const uint8_t* src;
+            int bytes = TILE_BYTES, parts = 2;
+            if (feed.is_full()) {
+                bool fresh = false;
+                const int id = feed.lookup(p, warp, lane, fresh);
+                if (id < 0) {
+                    feed.b += WARPS;
+                    continue;
+                }
+                src = (sub ? p.v_blocks : p.k_blocks) +
+                      (static_cast<int64_t>(id) * p.kv_heads + head) * TILE_BYTES;
+            } else {
+                const int left = feed.len % BLOCK;
+                const int halves = left > 32 ? 2 : 1;
+                parts = 2 * halves;
+                const int half = sub % halves;
+                src = reinterpret_cast<const uint8_t*>(sub < halves ? p.k_tail : p.v_tail) +
+                      (static_cast<int64_t>(feed.slot) * p.kv_heads + head) * (2 * TILE_BYTES) +
+                      half * TILE_BYTES;
+                bytes = min(left - 32 * half, 32) * D * 2;
+            }
+            if (lane == 0) {
+                const int s = fed % STAGES;
+                const uint32_t bar = smem_u32(&sm.full[warp][s]);
+                mbar_arrive_expect_tx(bar, bytes);
+                bulk_load(smem_u32(sm.ring[warp][s]), src, bytes, bar);
+            }
+            ++fed;
+            if (++sub == parts) {
+                sub = 0;
+                feed.b += WARPS;
+            }
+            return;
+        }
+    };
+    __syncwarp();
+    for (int s = 0; s < STAGES; ++s) request();
+
+    int stage = 0;                     // the next stage to read
+    uint32_t phase = 0;
+    bool alive = true;                 // no wait has given up
+    const auto await = [&](int ahead) {
+        const int s = stage + ahead;
+        const int slot = s >= STAGES ? s - STAGES : s;
+        const uint32_t parity = s >= STAGES ? phase ^ 1 : phase;
+        const uint32_t bar = smem_u32(&sm.full[warp][slot]);
+        if (alive && !mbar_try_wait(bar, parity)) {
+            const uint64_t t0 = globaltimer_ns();
+            while (alive && !mbar_try_wait(bar, parity))
+                if (globaltimer_ns() - t0 > FU_DEFAULT_TIMEOUT_NS) {
+                    report_status(p.status, FU_DEV_PIPELINE_TIMEOUT, W_ATTENTION);
+                    alive = false;
+                }
+        }
+        return sm.ring[warp][slot];
+    };
+    // The warp has read its oldest stage: fill it again.
+    const auto release = [&]() {
+        __syncwarp();
+        if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+        }
+        request();
+    };
+
+    while (walk.enter(p, sm.first, pairs, warp)) {
+        const int head = walk.pair / p.row_tiles;
+        const int row0 = walk.pair % p.row_tiles * 16; // first row (query head of the group)
+        const __nv_bfloat16* q = p.q + walk.i * p.q_stride + (head * p.group + row0) * D;
+        const int rows = min(p.group - row0, ROWS);
+        const int len = walk.len;
+
+        // q fragments: k step (c, s) covers dims 64 c + 16 t + 4 s .. + 3 of lane (g, t).
+        uint4 qb[H][4];                                // as it is, BF16
+        uint32_t qf[H][16];                            // f16, times 2^-e
+        Score<kMode> score[H];
+        const float raw = kMode & 1 ? 2.f * LOG2E * p.scale / p.softcap : p.scale * LOG2E;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int row = g + 8 * h;
+            const bool there = row < rows;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                qb[h][c] = there ? *reinterpret_cast<const uint4*>(
+                                       q + row * D + 64 * (c >> 1) + 16 * t + 8 * (c & 1))
+                                 : make_uint4(0, 0, 0, 0);
+            const uint32_t* w = &qb[h][0].x;
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[k])), fabsf(bf16_hi(w[k]))));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // q = (q 2^-e) 2^e with the row's largest value in [1, 2).
+            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+            const float down = __int_as_float((127 - e) << 23);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                qf[h][k] = pack_f16x2(bf16_lo(w[k]) * down, bf16_hi(w[k]) * down);
+            score[h].factor = raw * __int_as_float((127 + e) << 23);
+            score[h].cap_out = p.softcap * LOG2E;
+            score[h].slope = (kMode & 2) && there
+                                 ? __ldg(p.alibi_slopes + head * p.group + row0 + row) * LOG2E
+                                 : 0.f;
+        }
+
+        Rows<kWide> r;
+        r.clear();
+        float k_scales = 0.f, v_scales = 0.f;          // lane k: of the warp's k-th of 32 blocks
+        for (; walk.b < walk.b1; walk.b += WARPS) {
+            float s[H][8][2], old[H];
+            if (walk.is_full()) {
+                bool fresh;
+                const int id = walk.lookup(p, warp, lane, fresh);
+                if (fresh) {
+                    const int64_t at = static_cast<int64_t>(max(walk.id, 0)) * p.kv_heads + head;
+                    k_scales = __ldg(p.k_scales + at);
+                    v_scales = __ldg(p.v_scales + at);
+                }
+                if (id < 0) {
+                    report_status(p.status, FU_DEV_CACHE_RANGE, W_ATTENTION);
+                    continue;
+                }
+                const int k = (walk.b - walk.b0 - warp) / WARPS & 31;
+                const float ks = __shfl_sync(0xffffffffu, k_scales, k);
+                const float vs = __shfl_sync(0xffffffffu, v_scales, k);
+                const uint8_t* tile = await(0);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint8_t* row = tile + (16 * (g >> 1) + 2 * j + (g & 1)) * D + 16 * t;
+                    const uint4 x[2] = {*reinterpret_cast<const uint4*>(row),
+                                        *reinterpret_cast<const uint4*>(row + 64)};
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t w = (&x[k >> 2].x)[k & 3];
+                        const uint32_t a[4] = {qf[0][2 * k], kWide ? qf[H - 1][2 * k] : 0u,
+                                               qf[0][2 * k + 1],
+                                               kWide ? qf[H - 1][2 * k + 1] : 0u};
+                        mma_f16(acc, a, e4m3x2_to_f16x2<0>(w), e4m3x2_to_f16x2<1>(w));
+                    }
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            s[h][j][c] = score[h](
+                                acc[2 * h + c], ks,
+                                len - 1 - (walk.b * BLOCK + 16 * t + 2 * j + c));
+                }
+                release();
+                softmax_step<kWide>(r, s, old);
+                uint32_t pf[4][4];                     // weights of tokens 16 t + 4 k .. + 3
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        pf[k][2 * x] = pack_f16x2(s[0][2 * k + x][0], s[0][2 * k + x][1]);
+                        pf[k][2 * x + 1] =
+                            kWide ? pack_f16x2(s[H - 1][2 * k + x][0], s[H - 1][2 * k + x][1]) : 0u;
+                    }
+                tile = await(0);
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    const uint4 x =
+                        *reinterpret_cast<const uint4*>(tile + (16 * g + d) * BLOCK + 16 * t);
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t w = (&x.x)[k];
+                        mma_f16(acc, pf[k], e4m3x2_to_f16x2<0>(w), e4m3x2_to_f16x2<1>(w));
+                    }
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            r.o[h][d][c] = fmaf(acc[2 * h + c], vs, r.o[h][d][c] * old[h]);
+                }
+                release();
+                continue;
+            }
+
+            // The unfinished block; rows behind its last token are not read.
+            const int left = len % BLOCK;
+            const bool both = left > 32;
+            const uint8_t* tile = await(0);
+            const uint8_t* tile2 = both ? await(1) : tile;
+            const uint8_t* half = g < 4 ? tile : tile2 - TILE_BYTES;   // K rows from 32 on
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = 16 * (g >> 1) + 2 * j + (g & 1);
+                uint4 x[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    x[c] = row < left ? *reinterpret_cast<const uint4*>(
+                                            half + (row * D + 64 * (c >> 1) + 16 * t +
+                                                    8 * (c & 1)) * 2)
+                                      : make_uint4(0, 0, 0, 0);
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t* w = &x[k >> 1].x + 2 * (k & 1);
+                    const uint32_t* q0 = &qb[0][k >> 1].x + 2 * (k & 1);
+                    const uint32_t* q1 = &qb[H - 1][k >> 1].x + 2 * (k & 1);
+                    const uint32_t a[4] = {q0[0], kWide ? q1[0] : 0u, q0[1], kWide ? q1[1] : 0u};
+                    mma_bf16(acc, a, w[0], w[1]);
+                }
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    Score<kMode> plain = score[h];
+                    plain.factor = raw;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int token = 16 * t + 2 * j + c;
+                        const float x2 = plain(acc[2 * h + c], 1.f, left - 1 - token);
+                        s[h][j][c] = token < left ? x2 : -INFINITY;
+                    }
+                }
+            }
+            release();
+            if (both) release();
+            softmax_step<kWide>(r, s, old);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    r.o[h][d][0] *= old[h];
+                    r.o[h][d][1] *= old[h];
+                }
+            tile = await(0);
+            tile2 = both ? await(1) : tile;
+            half = t < 2 ? tile : tile2 - TILE_BYTES;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint4 x[4][2];                         // four tokens, dims 16 g .. 16 g + 15
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int row = 16 * t + 4 * k + y;
+                        x[y][c] = row < left ? *reinterpret_cast<const uint4*>(
+                                                   half + (row * D + 16 * g + 8 * c) * 2)
+                                             : make_uint4(0, 0, 0, 0);
+                    }
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h >= H) {
+                            hi[2 * y + h] = lo[2 * y + h] = 0u;
+                            continue;
+                        }
+                        const float w0 = s[h % H][2 * k + y][0], w1 = s[h % H][2 * k + y][1];
+                        const uint32_t top = pack_bf16x2(w0, w1);
+                        hi[2 * y + h] = top;
+                        lo[2 * y + h] = pack_bf16x2(w0 - bf16_lo(top), w1 - bf16_hi(top));
+                    }
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    const uint32_t sel = d & 1 ? 0x7632 : 0x5410;
+                    const uint32_t w0 = (&x[0][d >> 3].x)[(d & 7) >> 1];
+                    const uint32_t w1 = (&x[1][d >> 3].x)[(d & 7) >> 1];
+                    const uint32_t w2 = (&x[2][d >> 3].x)[(d & 7) >> 1];
+                    const uint32_t w3 = (&x[3][d >> 3].x)[(d & 7) >> 1];
+                    const uint32_t f0 = __byte_perm(w0, w1, sel), f1 = __byte_perm(w2, w3, sel);
+                    float acc[4] = {r.o[0][d][0], r.o[0][d][1], r.o[H - 1][d][0],
+                                    r.o[H - 1][d][1]};
+                    mma_bf16(acc, hi, f0, f1);
+                    mma_bf16(acc, lo, f0, f1);
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        r.o[h][d][0] = acc[2 * h];
+                        r.o[h][d][1] = acc[2 * h + 1];
+                    }
+                }
+            }
+            release();
+            if (both) release();
+        }
+
+        // Join the warps: warps 1 .. 3 leave theirs in shared memory, warp 0 adds
+        // them to its own, in order.
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 1);
+            r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 2);
+        }
+        if (warp > 0) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                float* dst = sm.o[warp - 1][g + 8 * h];
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int d = 0; d < 16; d += 4)
+                        *reinterpret_cast<float4*>(dst + 32 * t + 16 * c + d) =
+                            make_float4(r.o[h][d][c], r.o[h][d + 1][c], r.o[h][d + 2][c],
+                                        r.o[h][d + 3][c]);
+                if (t == 0) {
+                    dst[D] = r.m[h];
+                    dst[D + 1] = r.l[h];
+                }
+            }
+        }
+        __syncthreads();
+        if (warp == 0) {
+            const bool whole = walk.b1 - walk.b0 == walk.nb;
+            // A CTA has at most two pairs that it shares with others: the one it
+            // begins in (slot 0) and the one it ends in (slot 1 unless the same).
+            const bool at_begin = walk.at - (walk.b1 - walk.b0) == begin;
+            float* part = p.partial +
+                          (static_cast<int64_t>(blockIdx.x) * 2 + (at_begin ? 0 : 1)) * ROWS * PART;
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int row = g + 8 * h;
+                float top = r.m[h];
+#pragma unroll
+                for (int w = 0; w < WARPS - 1; ++w) top = fmaxf(top, sm.o[w][row][D]);
+                const float base = top == -INFINITY ? 0.f : top;
+                float f = ex2(r.m[h] - base), l = r.l[h] * f;
+#pragma unroll
+                for (int d = 0; d < 16; ++d) {
+                    r.o[h][d][0] *= f;
+                    r.o[h][d][1] *= f;
+                }
+#pragma unroll
+                for (int w = 0; w < WARPS - 1; ++w) {
+                    const float* src = sm.o[w][row];
+                    f = ex2(src[D] - base);
+                    l = fmaf(src[D + 1], f, l);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int d = 0; d < 16; d += 4) {
+                            const float4 x =
+                                *reinterpret_cast<const float4*>(src + 32 * t + 16 * c + d);
+                            r.o[h][d][c] = fmaf(x.x, f, r.o[h][d][c]);
+                            r.o[h][d + 1][c] = fmaf(x.y, f, r.o[h][d + 1][c]);
+                            r.o[h][d + 2][c] = fmaf(x.z, f, r.o[h][d + 2][c]);
+                            r.o[h][d + 3][c] = fmaf(x.w, f, r.o[h][d + 3][c]);
+                        }
+                }
+                if (row >= rows) continue;
+                if (whole) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    __nv_bfloat16* out = p.out + walk.i * p.out_stride +
+                                         (head * p.group + row0 + row) * D + 32 * t;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int d = 0; d < 16; d += 8) {
+                            uint4 x;
+                            uint32_t* w = &x.x;
+#pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                w[y] = pack_bf16x2(r.o[h][d + 2 * y][c] * inv,
+                                                   r.o[h][d + 2 * y + 1][c] * inv);
+                            *reinterpret_cast<uint4*>(out + 16 * c + d) = x;
+                        }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int d = 0; d < 16; d += 4)
+                            *reinterpret_cast<float4*>(part + row * PART + 32 * t + 16 * c + d) =
+                                make_float4(r.o[h][d][c], r.o[h][d + 1][c], r.o[h][d + 2][c],
+                                            r.o[h][d + 3][c]);
+                    if (t == 0) {
+                        part[row * PART + D] = top;
+                        part[row * PART + D + 1] = l;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // Nothing is in flight here unless a wait gave up: then the copies must
+    // land before shared memory is released.
+    if (!alive) {
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000) {
+        }
+    }
+}
+
+// One CTA per (sequence, pair): joins its partials, if it was split.
+__global__ void __launch_bounds__(D) attention_join_kernel(const AttentionParams p, int part_rows) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const int i = blockIdx.x, pair = blockIdx.y, d = threadIdx.x;
+    const int pairs = gridDim.y;
+    const int first = p.plan->first[i], share = p.plan->share;
+    const int nb = (p.plan->first[i + 1] - first) / pairs;
+    if (nb == 0) return;
+    // The CTAs that hold a part, and which of the first one's two partials it is.
+    int c0, c1, slot0 = 0;
+    if (p.plan->aligned) {
+        const int per = (nb + share - 1) / share;
+        c0 = p.plan->unit[i] + pair * per;
+        c1 = c0 + per;
+    } else {
+        const int a = first + pair * nb;
+        c0 = a / share;
+        c1 = (a + nb - 1) / share + 1;
+        slot0 = a == c0 * share ? 0 : 1;
+    }
+    if (c1 - c0 == 1) return;
+    const int head = pair / p.row_tiles, row0 = pair % p.row_tiles * 16;
+    const int rows = min(p.group - row0, part_rows);
+    for (int row = 0; row < rows; ++row) {
+        const auto part = [&](int c) {
+            return p.partial +
+                   ((static_cast<int64_t>(c) * 2 + (c == c0 ? slot0 : 0)) * part_rows + row) * PART;
+        };
+        float top = -INFINITY;
+        for (int c = c0; c < c1; ++c) top = fmaxf(top, part(c)[D]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float o = 0.f, l = 0.f;
+        for (int c = c0; c < c1; ++c) {
+            const float* x = part(c);
+            const float f = ex2(x[D] - base);
+            o = fmaf(f, x[d], o);
+            l = fmaf(f, x[D + 1], l);
+        }
+        p.out[i * p.out_stride + (head * p.group + row0 + row) * D + d] =
+            __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
+    }
 }
 
 // ------------------------------------------------------------ host side
@@ -400,10 +1111,22 @@ extern "C" int fu_kvcache_append(const fu_kvcache* c, const void* k, const void*
     return FU_OK;
 }
 
-extern "C" int64_t fu_kvcache_attention_workspace(int32_t, int32_t q_heads, int32_t kv_heads,
-                                                  int32_t seqs) {
+// CTAs of the split kernel: two per SM (its registers allow no more).
+static int split_ctas(int device) {
+    int sms = 0;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return 2 * sms;
+}
+
+extern "C" int64_t fu_kvcache_attention_workspace(int32_t device, int32_t q_heads,
+                                                  int32_t kv_heads, int32_t seqs) {
     if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || seqs < 1) return 0;
-    return 16;
+    const int rows = q_heads / kv_heads > 8 ? 16 : 8;
+    return static_cast<int64_t>(sizeof(kvcache::Plan)) +
+           static_cast<int64_t>(split_ctas(device)) * 2 * rows * kvcache::PART * 4;
 }
 
 extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t q_stride,
@@ -427,12 +1150,12 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
         workspace_bytes < fu_kvcache_attention_workspace(c->device, q_heads, c->kv_heads, seqs))
         return set_error(FU_ERR_INVALID, "workspace too small or not 16-byte aligned");
     kvcache::AttentionParams p = {};
-    p.blocks[0] = static_cast<const uint8_t*>(c->k_blocks);
-    p.blocks[1] = static_cast<const uint8_t*>(c->v_blocks);
-    p.scales[0] = c->k_scales;
-    p.scales[1] = c->v_scales;
-    p.tail[0] = static_cast<const __nv_bfloat16*>(c->k_tail);
-    p.tail[1] = static_cast<const __nv_bfloat16*>(c->v_tail);
+    p.k_blocks = static_cast<const uint8_t*>(c->k_blocks);
+    p.v_blocks = static_cast<const uint8_t*>(c->v_blocks);
+    p.k_scales = c->k_scales;
+    p.v_scales = c->v_scales;
+    p.k_tail = static_cast<const __nv_bfloat16*>(c->k_tail);
+    p.v_tail = static_cast<const __nv_bfloat16*>(c->v_tail);
     p.block_table = c->block_table;
     p.q = static_cast<const __nv_bfloat16*>(q);
     p.out = static_cast<__nv_bfloat16*>(out);
@@ -446,14 +1169,46 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
     p.num_blocks = c->num_blocks;
     p.max_seqs = c->max_seqs;
     p.max_blocks = c->max_blocks;
-    p.seqs = seqs;
     p.group = q_heads / c->kv_heads;
+    p.row_tiles = (p.group + 15) / 16;
+    p.plan = static_cast<kvcache::Plan*>(workspace);
+    p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + sizeof(kvcache::Plan));
+    p.ctas = split_ctas(c->device);
+    const int64_t per_seq = static_cast<int64_t>(c->max_blocks) * c->kv_heads * p.row_tiles;
+    if (per_seq > INT32_MAX)
+        return set_error(FU_ERR_INVALID, "max_blocks * kv_heads is too large for one call");
+    const int64_t batch = std::min<int64_t>(kvcache::MAX_BATCH, INT32_MAX / per_seq);
     p.scale = scale;
     p.softcap = softcap;
     DeviceGuard guard(c->device);
     if (!guard.ok()) return set_error(FU_ERR_INVALID, "device %d is not available", c->device);
-    Launch launch(dim3(seqs, q_heads), dim3(32), 0, stream, (flags & FU_FWD_NO_PDL) == 0);
-    cudaError_t e = cudaLaunchKernelEx(&launch.cfg, kvcache::attention_kernel, p);
-    if (e != cudaSuccess) return set_error(FU_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    const bool wide = p.group > 8, pdl = (flags & FU_FWD_NO_PDL) == 0;
+    const int mode = (softcap > 0.f ? 1 : 0) | (alibi_slopes != nullptr ? 2 : 0);
+    void (*const kernels[2][4])(kvcache::AttentionParams) = {
+        {kvcache::attention_split_kernel<false, 0>, kvcache::attention_split_kernel<false, 1>,
+         kvcache::attention_split_kernel<false, 2>, kvcache::attention_split_kernel<false, 3>},
+        {kvcache::attention_split_kernel<true, 0>, kvcache::attention_split_kernel<true, 1>,
+         kvcache::attention_split_kernel<true, 2>, kvcache::attention_split_kernel<true, 3>}};
+    const int smem = wide ? sizeof(kvcache::SplitSmem<true>) : sizeof(kvcache::SplitSmem<false>);
+    cudaError_t e = cudaFuncSetAttribute(kernels[wide][mode],
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess)
+        return set_error(FU_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    for (int64_t done = 0; done < seqs; done += batch) {
+        p.seqs = static_cast<int32_t>(std::min(seqs - done, batch));
+        p.q = static_cast<const __nv_bfloat16*>(q) + done * q_stride;
+        p.out = static_cast<__nv_bfloat16*>(out) + done * out_stride;
+        p.slots = slots + done;
+        p.seq_lens = seq_lens + done;
+        Launch split(dim3(p.ctas), dim3(kvcache::SPLIT_THREADS), smem, stream, pdl);
+        e = cudaLaunchKernelEx(&split.cfg, kernels[wide][mode], p);
+        if (e == cudaSuccess) {
+            Launch join(dim3(p.seqs, c->kv_heads * p.row_tiles), dim3(kvcache::D), 0, stream, pdl);
+            e = cudaLaunchKernelEx(&join.cfg, kvcache::attention_join_kernel,
+                                   static_cast<const kvcache::AttentionParams>(p), wide ? 16 : 8);
+        }
+        if (e != cudaSuccess)
+            return set_error(FU_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
+    }
     return FU_OK;
 }
