@@ -238,11 +238,16 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 // the cache bounds it (256 bytes per token and head), so the work is split
 // along the tokens over all SMs and joined afterwards:
 //
-//   attention_split_kernel   CTAs of 4 warps; a warp takes whole blocks, with
-//                            an online softmax of its own; the CTA joins its
-//                            warps and writes either the output or a partial
+//   attention_split_kernel   every warp takes a share of whole blocks, with an
+//                            online softmax of its own, and writes the output
+//                            of a (sequence, head) that it had all of, or a
+//                            partial
 //   attention_join_kernel    joins the partials of split (sequence, head)s,
 //                            in their order, so results do not depend on timing
+//
+// Warps work alone: a CTA that joined its four warps at the end of each
+// (sequence, head) lost 5 to 8 us there to the chain of loads and barriers
+// (64 sequences of up to 8192 tokens, 8 K/V heads: 134 us).
 //
 // A block is two contiguous 8 KiB tiles (K, V transposed), which each warp has
 // copied into a ring of its own in shared memory (cp.async.bulk), across the
@@ -265,7 +270,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 // weights as a sum of two BF16 so that they keep 16 bits.
 constexpr int WARPS = 4;
 constexpr int SPLIT_THREADS = 32 * WARPS;
-constexpr int MAX_BATCH = 512;         // sequences per launch (their prefix sums sit in shared memory)
+constexpr int MAX_BATCH = 1024;        // sequences per launch (their prefix sums sit in shared memory)
 constexpr int TILE_BYTES = BLOCK * D;  // one stage of a warp's ring: K or V of a block
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -285,40 +290,38 @@ struct AttentionParams {
     const float* alibi_slopes;
     int32_t* status;
     struct Plan* plan;
-    float* partial;                    // [CTA][2][rows of a unit][PART]
-    int32_t kv_heads, num_blocks, max_seqs, max_blocks, seqs, group, row_tiles, ctas;
+    float* partial;                    // [worker][2][rows of a pair][PART]
+    int32_t kv_heads, num_blocks, max_seqs, max_blocks, seqs, group, row_tiles;
+    int32_t workers;                   // warps of the split kernel
     float scale, softcap;
 };
 constexpr int PART = D + 4;            // one row of a partial: 128 sums, m, l, padding
 
-// How the call's blocks are dealt to the CTAs.  The items are the blocks of
+// How the call's blocks are dealt to the warps.  The items are the blocks of
 // all (sequence, K/V head, row tile)s -- pairs -- one after another; sequence
 // i's begin at first[i], nb blocks for each of its pairs.
-//   aligned (few pairs): a CTA takes up to `share` blocks of one pair; the
+//   aligned (few pairs): a warp takes up to `share` blocks of one pair; the
 //     units of sequence i begin at unit[i] = sum of ceil(nb / share) * pairs.
-//   otherwise a CTA takes `share` consecutive items, of as many pairs as that is.
+//   otherwise a warp takes `share` consecutive items, of as many pairs as that is.
 struct alignas(16) Plan {
     int32_t items, share, aligned, pad;
     int32_t first[MAX_BATCH + 1];
     int32_t unit[MAX_BATCH + 1];
 };
-
 static_assert(sizeof(Plan) % 16 == 0, "the partials behind it are written 16 bytes at a time");
 
 // Shared memory of a split CTA.  Three stages a warp put 192 KiB per SM in
-// flight; the wide rows' joining area leaves room for two.
-template <bool kWide>
+// flight.
+constexpr int STAGES = 3;
 struct SplitSmem {
-    static constexpr int STAGES = kWide ? 2 : 3, ROWS = kWide ? 16 : 8;
     uint8_t ring[WARPS][STAGES][TILE_BYTES];
-    float o[WARPS - 1][ROWS][PART];
     uint64_t full[WARPS][STAGES];
-    int32_t first[MAX_BATCH + 1];
-    int32_t unit[MAX_BATCH / 4 + 1];
+    float scale[WARPS][STAGES];        // of the stage's block
+    int32_t first[MAX_BATCH + 1], unit[MAX_BATCH + 1];      // as in Plan
+    int32_t slot[MAX_BATCH], len[MAX_BATCH];
     int32_t scan[WARPS];
 };
-static_assert(2 * (sizeof(SplitSmem<false>) + 1024) <= 228 * 1024, "two CTAs per SM");
-static_assert(2 * (sizeof(SplitSmem<true>) + 1024) <= 228 * 1024, "two CTAs per SM");
+static_assert(2 * (sizeof(SplitSmem) + 1024) <= 228 * 1024, "two CTAs per SM");
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
@@ -369,6 +372,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                                           uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes "
                  "[%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+// Four bytes, counted on `bar` as one arrival when they are there.
+__device__ __forceinline__ void async_load_4(uint32_t dst, const void* src, uint32_t bar) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n\t"
+                 "cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%2];"
+                 ::"r"(dst), "l"(src), "r"(bar) : "memory");
 }
 
 // A warp's running softmax and output for its rows: row g (and g + 8 if kWide).
@@ -431,41 +441,45 @@ __device__ __forceinline__ void softmax_step(Rows<kWide>& r, float (&s)[Rows<kWi
     }
 }
 
-// A warp's way through its CTA's items [at, end): pair by pair, within a pair
-// every WARPS-th block.  The feed of the ring and the arithmetic each have one.
-struct Walk {
-    int at, end;                       // items of the CTA not entered yet
-    int i, pair, b0, b1, nb;           // the current pair, its blocks here [b0, b1) of nb
-    int slot, len, b;                  // b: the warp's current block
-    int id;                            // lane k: cache block of the warp's k-th of 32 blocks
+// The last i in [0, n) with x[i] <= v (x does not decrease, x[0] <= v).
+__device__ __forceinline__ int last_at_or_before(const int32_t* x, int n, int v) {
+    int i = 0;
+    while (n - i > 1) {
+        const int mid = (i + n) >> 1;
+        if (x[mid] <= v) i = mid; else n = mid;
+    }
+    return i;
+}
 
-    __device__ bool enter(const AttentionParams& p, const int32_t* first, int pairs, int warp) {
+// A way through a warp's items [at, end), pair by pair.  The feed of the ring
+// and the arithmetic each have one.
+struct Walk {
+    int at, end;                       // items not entered yet
+    int i, pair, b0, b1, nb;           // the current pair, its blocks here [b0, b1) of nb
+    int slot, len, b;                  // b: the current block
+    int id;                            // lane k: cache block of the k-th of 32 blocks
+
+    __device__ bool enter(const SplitSmem& sm, int pairs) {
         if (at >= end) return false;
-        i = 0;                         // the last sequence that begins at `at` or before
-        for (int hi = p.seqs; hi - i > 1;) {
-            const int mid = (i + hi) >> 1;
-            if (first[mid] <= at) i = mid; else hi = mid;
-        }
-        nb = (first[i + 1] - first[i]) / pairs;
-        pair = (at - first[i]) / nb;
-        b0 = at - first[i] - pair * nb;
+        while (sm.first[i + 1] <= at) ++i;
+        slot = sm.slot[i];
+        len = sm.len[i];
+        nb = (len + BLOCK - 1) / BLOCK;
+        pair = (at - sm.first[i]) / nb;
+        b = b0 = at - sm.first[i] - pair * nb;
         b1 = min(nb, b0 + end - at);
         at += b1 - b0;
-        slot = __ldg(p.slots + i);
-        len = __ldg(p.seq_lens + i);
-        b = b0 + warp;
         return true;
     }
     __device__ bool is_full() const { return b < len / BLOCK; }
     // Cache block of block b (a full one), -1 if it is outside the cache.  The
-    // warp looks up 32 at a time; `fresh` says that it just did.
-    __device__ int lookup(const AttentionParams& p, int warp, int lane, bool& fresh) {
-        const int k = (b - b0 - warp) / WARPS & 31;
-        fresh = k == 0;
-        if (fresh) {
-            const int mine = b + WARPS * lane;
-            id = mine < min(b1, len / BLOCK)
-                     ? __ldg(p.block_table + static_cast<int64_t>(slot) * p.max_blocks + mine) : 0;
+    // warp looks up 32 at a time.
+    __device__ int lookup(const AttentionParams& p, int lane) {
+        const int k = (b - b0) & 31;
+        if (k == 0) {
+            id = b + lane < min(b1, len / BLOCK)
+                     ? __ldg(p.block_table + static_cast<int64_t>(slot) * p.max_blocks + b + lane)
+                     : 0;
             if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.num_blocks)) id = -1;
         }
         return __shfl_sync(0xffffffffu, id, k);
@@ -475,14 +489,13 @@ struct Walk {
 template <bool kWide, int kMode>
 __global__ void __launch_bounds__(SPLIT_THREADS, 2)
 attention_split_kernel(const AttentionParams p) {
-    using Smem = SplitSmem<kWide>;
-    constexpr int H = Rows<kWide>::H, ROWS = 8 * H, STAGES = Smem::STAGES;
+    constexpr int H = Rows<kWide>::H, ROWS = 8 * H;
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    SplitSmem& sm = *reinterpret_cast<SplitSmem*>(smem_raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     if (lane == 0) {
-        for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&sm.full[warp][s]), 1);
+        for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&sm.full[warp][s]), 2);
         fence_mbar_init();
     }
     grid_dependency_wait();
@@ -491,12 +504,32 @@ attention_split_kernel(const AttentionParams p) {
     // Prefix sums of the sequences' blocks; a row that is padding or does not
     // fit has none.
     const int pairs = p.kv_heads * p.row_tiles;
+    // Sum of x over the threads before this one; adds all of them to `total`.
+    const auto scan = [&](int x, int& total) {
+        int sum = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += up;
+        }
+        if (lane == 31) sm.scan[warp] = sum;
+        __syncthreads();
+        int before = total;
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) before += sm.scan[w];
+            total += sm.scan[w];
+        }
+        __syncthreads();
+        return before + sum - x;
+    };
     int total = 0;
     for (int i0 = 0; i0 < p.seqs; i0 += SPLIT_THREADS) {
         const int i = i0 + threadIdx.x;
         int nb = 0;
         if (i < p.seqs) {
             const int slot = __ldg(p.slots + i), len = __ldg(p.seq_lens + i);
+            sm.slot[i] = slot;
+            sm.len[i] = len;
             if (slot >= 0) {
                 if (slot >= p.max_seqs || len < 0 || len > p.max_blocks * BLOCK) {
                     if (blockIdx.x == 0)
@@ -513,42 +546,29 @@ attention_split_kernel(const AttentionParams p) {
                 }
             }
         }
-        int sum = nb;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += up;
-        }
-        if (lane == 31) sm.scan[warp] = sum;
-        __syncthreads();
-        int before = total;
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) before += sm.scan[w];
-            total += sm.scan[w];
-        }
-        if (i < p.seqs) sm.first[i] = (before + sum - nb) * pairs;
-        __syncthreads();
+        const int before = scan(nb, total);
+        if (i < p.seqs) sm.first[i] = before * pairs;
     }
     const int items = total * pairs;
     if (threadIdx.x == 0) sm.first[p.seqs] = items;
-    // Few pairs: each is cut into shares of its own, a multiple of WARPS blocks,
-    // that give at most one to every CTA; else the items are dealt evenly.
+    // Few pairs: each is cut into shares of its own that give at most one to
+    // every warp; else the items are dealt evenly.
     const int all_pairs = p.seqs * pairs;
-    const bool aligned = all_pairs <= p.ctas / 4;
-    const int over = aligned ? p.ctas - all_pairs : p.ctas;
-    const int each = items / over + (items % over != 0);
-    const int share = max((each + WARPS - 1) / WARPS * WARPS, WARPS);
+    const bool aligned = all_pairs <= p.workers / 4;
+    const int over = aligned ? p.workers - all_pairs : p.workers;
+    const int share = max(items / over + (items % over != 0), 1);
     __syncthreads();
-    if (aligned && threadIdx.x == 0) {
+    if (aligned) {
         int units = 0;
-        for (int i = 0; i < p.seqs; ++i) {
-            sm.unit[i] = units;
-            const int nb = (sm.first[i + 1] - sm.first[i]) / pairs;
-            units += (nb + share - 1) / share * pairs;
+        for (int i0 = 0; i0 < p.seqs; i0 += SPLIT_THREADS) {
+            const int i = i0 + threadIdx.x;
+            const int nb = i < p.seqs ? (sm.first[i + 1] - sm.first[i]) / pairs : 0;
+            const int before = scan((nb + share - 1) / share * pairs, units);
+            if (i < p.seqs) sm.unit[i] = before;
         }
-        sm.unit[p.seqs] = units;
+        if (threadIdx.x == 0) sm.unit[p.seqs] = units;
+        __syncthreads();
     }
-    __syncthreads();
     if (blockIdx.x == 0) {
         for (int i = threadIdx.x; i <= p.seqs; i += SPLIT_THREADS) {
             p.plan->first[i] = sm.first[i];
@@ -561,21 +581,23 @@ attention_split_kernel(const AttentionParams p) {
         }
     }
 
-    // This CTA's items [at, end), pair by pair.
+    // This warp's items.  Neighbours in the order of the items are on different SMs.
+    const int worker = warp * gridDim.x + blockIdx.x;
     Walk walk = {};
     if (aligned) {
-        const int u = blockIdx.x;
-        if (u >= sm.unit[p.seqs]) return;
-        int i = 0;
-        while (sm.unit[i + 1] <= u) ++i;
-        const int nb = (sm.first[i + 1] - sm.first[i]) / pairs;
+        if (worker >= sm.unit[p.seqs]) return;
+        walk.i = last_at_or_before(sm.unit, p.seqs, worker);
+        const int first = sm.first[walk.i], nb = (sm.first[walk.i + 1] - first) / pairs;
         const int per = (nb + share - 1) / share;
-        const int pair = (u - sm.unit[i]) / per, part = (u - sm.unit[i]) % per;
-        walk.at = sm.first[i] + pair * nb + part * share;
-        walk.end = min(walk.at + share, sm.first[i] + (pair + 1) * nb);
+        const int pair = (worker - sm.unit[walk.i]) / per;
+        walk.at = first + pair * nb + (worker - sm.unit[walk.i]) % per * share;
+        walk.end = min(walk.at + share, first + (pair + 1) * nb);
     } else {
-        walk.at = min(static_cast<int64_t>(blockIdx.x) * share, static_cast<int64_t>(items));
-        walk.end = min(walk.at + static_cast<int64_t>(share), static_cast<int64_t>(items));
+        const int64_t at = static_cast<int64_t>(worker) * share;
+        if (at >= items) return;
+        walk.at = static_cast<int>(at);
+        walk.end = static_cast<int>(min(at + share, static_cast<int64_t>(items)));
+        walk.i = last_at_or_before(sm.first, p.seqs, walk.at);
     }
     const int begin = walk.at;
 
@@ -584,10 +606,10 @@ attention_split_kernel(const AttentionParams p) {
     // halves of K, then of V.
     Walk feed = walk;
     bool feeding = false;
-    int sub = 0, fed = 0;              // part of the current block; stages requested so far
+    int sub = 0, fed = 0;              // part of the current block; the stage to fill next
     const auto request = [&]() {
         while (true) {
-            if (!feeding && !feed.enter(p, sm.first, pairs, warp)) return;
+            if (!feeding && !feed.enter(sm, pairs)) return;
             feeding = true;
             if (feed.b >= feed.b1) {
                 feeding = false;
@@ -595,16 +617,17 @@ attention_split_kernel(const AttentionParams p) {
             }
             const int head = feed.pair / p.row_tiles;
             const uint8_t* src;
+            const float* scale = nullptr;
             int bytes = TILE_BYTES, parts = 2;
             if (feed.is_full()) {
-                bool fresh = false;
-                const int id = feed.lookup(p, warp, lane, fresh);
+                const int id = feed.lookup(p, lane);
                 if (id < 0) {
-                    feed.b += WARPS;
+                    ++feed.b;
                     continue;
                 }
-                src = (sub ? p.v_blocks : p.k_blocks) +
-                      (static_cast<int64_t>(id) * p.kv_heads + head) * TILE_BYTES;
+                const int64_t block = static_cast<int64_t>(id) * p.kv_heads + head;
+                src = (sub ? p.v_blocks : p.k_blocks) + block * TILE_BYTES;
+                scale = (sub ? p.v_scales : p.k_scales) + block;
             } else {
                 const int left = feed.len % BLOCK;
                 const int halves = left > 32 ? 2 : 1;
@@ -616,15 +639,18 @@ attention_split_kernel(const AttentionParams p) {
                 bytes = min(left - 32 * half, 32) * D * 2;
             }
             if (lane == 0) {
-                const int s = fed % STAGES;
-                const uint32_t bar = smem_u32(&sm.full[warp][s]);
+                const uint32_t bar = smem_u32(&sm.full[warp][fed]);
                 mbar_arrive_expect_tx(bar, bytes);
-                bulk_load(smem_u32(sm.ring[warp][s]), src, bytes, bar);
+                bulk_load(smem_u32(sm.ring[warp][fed]), src, bytes, bar);
+                if (scale != nullptr)
+                    async_load_4(smem_u32(&sm.scale[warp][fed]), scale, bar);
+                else
+                    mbar_arrive(bar);
             }
-            ++fed;
+            fed = fed + 1 == STAGES ? 0 : fed + 1;
             if (++sub == parts) {
                 sub = 0;
-                feed.b += WARPS;
+                ++feed.b;
             }
             return;
         }
@@ -660,7 +686,7 @@ attention_split_kernel(const AttentionParams p) {
         request();
     };
 
-    while (walk.enter(p, sm.first, pairs, warp)) {
+    while (walk.enter(sm, pairs)) {
         const int head = walk.pair / p.row_tiles;
         const int row0 = walk.pair % p.row_tiles * 16; // first row (query head of the group)
         const __nv_bfloat16* q = p.q + walk.i * p.q_stride + (head * p.group + row0) * D;
@@ -703,25 +729,15 @@ attention_split_kernel(const AttentionParams p) {
 
         Rows<kWide> r;
         r.clear();
-        float k_scales = 0.f, v_scales = 0.f;          // lane k: of the warp's k-th of 32 blocks
-        for (; walk.b < walk.b1; walk.b += WARPS) {
+        for (; walk.b < walk.b1; ++walk.b) {
             float s[H][8][2], old[H];
             if (walk.is_full()) {
-                bool fresh;
-                const int id = walk.lookup(p, warp, lane, fresh);
-                if (fresh) {
-                    const int64_t at = static_cast<int64_t>(max(walk.id, 0)) * p.kv_heads + head;
-                    k_scales = __ldg(p.k_scales + at);
-                    v_scales = __ldg(p.v_scales + at);
-                }
-                if (id < 0) {
+                if (walk.lookup(p, lane) < 0) {
                     report_status(p.status, FU_DEV_CACHE_RANGE, W_ATTENTION);
                     continue;
                 }
-                const int k = (walk.b - walk.b0 - warp) / WARPS & 31;
-                const float ks = __shfl_sync(0xffffffffu, k_scales, k);
-                const float vs = __shfl_sync(0xffffffffu, v_scales, k);
                 const uint8_t* tile = await(0);
+                const float ks = sm.scale[warp][stage];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint8_t* row = tile + (16 * (g >> 1) + 2 * j + (g & 1)) * D + 16 * t;
@@ -756,6 +772,7 @@ attention_split_kernel(const AttentionParams p) {
                             kWide ? pack_f16x2(s[H - 1][2 * k + x][0], s[H - 1][2 * k + x][1]) : 0u;
                     }
                 tile = await(0);
+                const float vs = sm.scale[warp][stage];
 #pragma unroll
                 for (int d = 0; d < 16; ++d) {
                     const uint4 x =
@@ -875,101 +892,49 @@ attention_split_kernel(const AttentionParams p) {
             if (both) release();
         }
 
-        // Join the warps: warps 1 .. 3 leave theirs in shared memory, warp 0 adds
-        // them to its own, in order.
+        const bool whole = walk.b1 - walk.b0 == walk.nb;
+        // A warp has at most two pairs that it shares with others: the one it
+        // begins in (slot 0) and the one it ends in (slot 1 unless the same).
+        const bool at_begin = walk.at - (walk.b1 - walk.b0) == begin;
+        float* part =
+            p.partial + (static_cast<int64_t>(worker) * 2 + (at_begin ? 0 : 1)) * ROWS * PART;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 1);
-            r.l[h] += __shfl_xor_sync(0xffffffffu, r.l[h], 2);
-        }
-        if (warp > 0) {
+            const int row = g + 8 * h;
+            float l = r.l[h];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (row >= rows) continue;
+            if (whole) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                __nv_bfloat16* out = p.out + walk.i * p.out_stride +
+                                     (head * p.group + row0 + row) * D + 32 * t;
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                float* dst = sm.o[warp - 1][g + 8 * h];
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int d = 0; d < 16; d += 8) {
+                        uint4 x;
+                        uint32_t* w = &x.x;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                            w[y] = pack_bf16x2(r.o[h][d + 2 * y][c] * inv,
+                                               r.o[h][d + 2 * y + 1][c] * inv);
+                        *reinterpret_cast<uint4*>(out + 16 * c + d) = x;
+                    }
+            } else {
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int d = 0; d < 16; d += 4)
-                        *reinterpret_cast<float4*>(dst + 32 * t + 16 * c + d) =
+                        *reinterpret_cast<float4*>(part + row * PART + 32 * t + 16 * c + d) =
                             make_float4(r.o[h][d][c], r.o[h][d + 1][c], r.o[h][d + 2][c],
                                         r.o[h][d + 3][c]);
                 if (t == 0) {
-                    dst[D] = r.m[h];
-                    dst[D + 1] = r.l[h];
+                    part[row * PART + D] = r.m[h];
+                    part[row * PART + D + 1] = l;
                 }
             }
         }
-        __syncthreads();
-        if (warp == 0) {
-            const bool whole = walk.b1 - walk.b0 == walk.nb;
-            // A CTA has at most two pairs that it shares with others: the one it
-            // begins in (slot 0) and the one it ends in (slot 1 unless the same).
-            const bool at_begin = walk.at - (walk.b1 - walk.b0) == begin;
-            float* part = p.partial +
-                          (static_cast<int64_t>(blockIdx.x) * 2 + (at_begin ? 0 : 1)) * ROWS * PART;
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                const int row = g + 8 * h;
-                float top = r.m[h];
-#pragma unroll
-                for (int w = 0; w < WARPS - 1; ++w) top = fmaxf(top, sm.o[w][row][D]);
-                const float base = top == -INFINITY ? 0.f : top;
-                float f = ex2(r.m[h] - base), l = r.l[h] * f;
-#pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                    r.o[h][d][0] *= f;
-                    r.o[h][d][1] *= f;
-                }
-#pragma unroll
-                for (int w = 0; w < WARPS - 1; ++w) {
-                    const float* src = sm.o[w][row];
-                    f = ex2(src[D] - base);
-                    l = fmaf(src[D + 1], f, l);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int d = 0; d < 16; d += 4) {
-                            const float4 x =
-                                *reinterpret_cast<const float4*>(src + 32 * t + 16 * c + d);
-                            r.o[h][d][c] = fmaf(x.x, f, r.o[h][d][c]);
-                            r.o[h][d + 1][c] = fmaf(x.y, f, r.o[h][d + 1][c]);
-                            r.o[h][d + 2][c] = fmaf(x.z, f, r.o[h][d + 2][c]);
-                            r.o[h][d + 3][c] = fmaf(x.w, f, r.o[h][d + 3][c]);
-                        }
-                }
-                if (row >= rows) continue;
-                if (whole) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    __nv_bfloat16* out = p.out + walk.i * p.out_stride +
-                                         (head * p.group + row0 + row) * D + 32 * t;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int d = 0; d < 16; d += 8) {
-                            uint4 x;
-                            uint32_t* w = &x.x;
-#pragma unroll
-                            for (int y = 0; y < 4; ++y)
-                                w[y] = pack_bf16x2(r.o[h][d + 2 * y][c] * inv,
-                                                   r.o[h][d + 2 * y + 1][c] * inv);
-                            *reinterpret_cast<uint4*>(out + 16 * c + d) = x;
-                        }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int d = 0; d < 16; d += 4)
-                            *reinterpret_cast<float4*>(part + row * PART + 32 * t + 16 * c + d) =
-                                make_float4(r.o[h][d][c], r.o[h][d + 1][c], r.o[h][d + 2][c],
-                                            r.o[h][d + 3][c]);
-                    if (t == 0) {
-                        part[row * PART + D] = top;
-                        part[row * PART + D + 1] = l;
-                    }
-                }
-            }
-        }
-        __syncthreads();
     }
     // Nothing is in flight here unless a wait gave up: then the copies must
     // land before shared memory is released.
@@ -980,20 +945,30 @@ attention_split_kernel(const AttentionParams p) {
     }
 }
 
-// One CTA per (sequence, pair): joins its partials, if it was split.
-__global__ void __launch_bounds__(D) attention_join_kernel(const AttentionParams p, int part_rows) {
+// One CTA per (sequence, pair, row): joins the row's partials, if the pair was
+// split.  Each warp takes every kThreads / 32th partial, four dims a lane, eight
+// in flight, with a running maximum; the warps' results are joined in order.
+// Few pairs have many partials each (512 threads), many pairs have few (128).
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads)
+attention_join_kernel(const AttentionParams p, int part_rows) {
+    constexpr int JOIN_WARPS = kThreads / 32, DEEP = 8;
+    __shared__ float s_m[JOIN_WARPS], s_l[JOIN_WARPS];
+    __shared__ float4 s_o[JOIN_WARPS][32];
     grid_dependency_wait();
     grid_launch_dependents();
-    const int i = blockIdx.x, pair = blockIdx.y, d = threadIdx.x;
-    const int pairs = gridDim.y;
-    const int first = p.plan->first[i], share = p.plan->share;
-    const int nb = (p.plan->first[i + 1] - first) / pairs;
+    const int i = blockIdx.x, pair = blockIdx.y, row = blockIdx.z, pairs = gridDim.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int first = p.plan->first[i], after = p.plan->first[i + 1], share = p.plan->share;
+    const int aligned = p.plan->aligned, unit = p.plan->unit[i];
+    const int nb = (after - first) / pairs;
     if (nb == 0) return;
-    // The CTAs that hold a part, and which of the first one's two partials it is.
+    // The warps of the split that hold a part, and which of the first one's two
+    // partials it is.
     int c0, c1, slot0 = 0;
-    if (p.plan->aligned) {
+    if (aligned) {
         const int per = (nb + share - 1) / share;
-        c0 = p.plan->unit[i] + pair * per;
+        c0 = unit + pair * per;
         c1 = c0 + per;
     } else {
         const int a = first + pair * nb;
@@ -1003,25 +978,73 @@ __global__ void __launch_bounds__(D) attention_join_kernel(const AttentionParams
     }
     if (c1 - c0 == 1) return;
     const int head = pair / p.row_tiles, row0 = pair % p.row_tiles * 16;
-    const int rows = min(p.group - row0, part_rows);
-    for (int row = 0; row < rows; ++row) {
-        const auto part = [&](int c) {
-            return p.partial +
-                   ((static_cast<int64_t>(c) * 2 + (c == c0 ? slot0 : 0)) * part_rows + row) * PART;
-        };
-        float top = -INFINITY;
-        for (int c = c0; c < c1; ++c) top = fmaxf(top, part(c)[D]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float o = 0.f, l = 0.f;
-        for (int c = c0; c < c1; ++c) {
-            const float* x = part(c);
-            const float f = ex2(x[D] - base);
-            o = fmaf(f, x[d], o);
-            l = fmaf(f, x[D + 1], l);
+    if (row0 + row >= p.group) return;
+
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -INFINITY, l = 0.f;
+    for (int c = c0 + warp; c < c1; c += DEEP * JOIN_WARPS) {
+        float4 x[DEEP];
+        float pm[DEEP], pl[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+            const int at = c + k * JOIN_WARPS;
+            pm[k] = -INFINITY;
+            pl[k] = 0.f;
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at < c1) {
+                const float* src = p.partial + ((static_cast<int64_t>(at) * 2 +
+                                                 (at == c0 ? slot0 : 0)) * part_rows + row) * PART;
+                x[k] = *reinterpret_cast<const float4*>(src + 4 * lane);
+                pm[k] = src[D];
+                pl[k] = src[D + 1];
+            }
         }
-        p.out[i * p.out_stride + (head * p.group + row0 + row) * D + d] =
-            __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) top = fmaxf(top, pm[k]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float f = ex2(m - base);
+        m = top;
+        l *= f;
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+            f = ex2(pm[k] - base);
+            l = fmaf(pl[k], f, l);
+            o.x = fmaf(x[k].x, f, o.x);
+            o.y = fmaf(x[k].y, f, o.y);
+            o.z = fmaf(x[k].z, f, o.z);
+            o.w = fmaf(x[k].w, f, o.w);
+        }
     }
+    s_o[warp][lane] = o;
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+    }
+    __syncthreads();
+    if (warp > 0) return;
+    float top = m;
+#pragma unroll
+    for (int w = 1; w < JOIN_WARPS; ++w) top = fmaxf(top, s_m[w]);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float f0 = ex2(m - base);
+    l *= f0;
+    o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+    for (int w = 1; w < JOIN_WARPS; ++w) {
+        const float4 x = s_o[w][lane];
+        const float f = ex2(s_m[w] - base);
+        l = fmaf(s_l[w], f, l);
+        o.x = fmaf(x.x, f, o.x);
+        o.y = fmaf(x.y, f, o.y);
+        o.z = fmaf(x.z, f, o.z);
+        o.w = fmaf(x.w, f, o.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(p.out + i * p.out_stride + (head * p.group + row0 + row) * D +
+                              4 * lane) =
+        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
 }
 
 // ------------------------------------------------------------ host side
@@ -1111,7 +1134,7 @@ extern "C" int fu_kvcache_append(const fu_kvcache* c, const void* k, const void*
     return FU_OK;
 }
 
-// CTAs of the split kernel: two per SM (its registers allow no more).
+// CTAs of the split kernel: two per SM (its shared memory allows no more).
 static int split_ctas(int device) {
     int sms = 0;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
@@ -1126,7 +1149,8 @@ extern "C" int64_t fu_kvcache_attention_workspace(int32_t device, int32_t q_head
     if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads || seqs < 1) return 0;
     const int rows = q_heads / kv_heads > 8 ? 16 : 8;
     return static_cast<int64_t>(sizeof(kvcache::Plan)) +
-           static_cast<int64_t>(split_ctas(device)) * 2 * rows * kvcache::PART * 4;
+           static_cast<int64_t>(split_ctas(device)) * kvcache::WARPS * 2 * rows *
+               kvcache::PART * 4;
 }
 
 extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t q_stride,
@@ -1173,7 +1197,8 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
     p.row_tiles = (p.group + 15) / 16;
     p.plan = static_cast<kvcache::Plan*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + sizeof(kvcache::Plan));
-    p.ctas = split_ctas(c->device);
+    const int ctas = split_ctas(c->device);
+    p.workers = ctas * kvcache::WARPS;
     const int64_t per_seq = static_cast<int64_t>(c->max_blocks) * c->kv_heads * p.row_tiles;
     if (per_seq > INT32_MAX)
         return set_error(FU_ERR_INVALID, "max_blocks * kv_heads is too large for one call");
@@ -1189,7 +1214,7 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
          kvcache::attention_split_kernel<false, 2>, kvcache::attention_split_kernel<false, 3>},
         {kvcache::attention_split_kernel<true, 0>, kvcache::attention_split_kernel<true, 1>,
          kvcache::attention_split_kernel<true, 2>, kvcache::attention_split_kernel<true, 3>}};
-    const int smem = wide ? sizeof(kvcache::SplitSmem<true>) : sizeof(kvcache::SplitSmem<false>);
+    const int smem = sizeof(kvcache::SplitSmem);
     cudaError_t e = cudaFuncSetAttribute(kernels[wide][mode],
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
@@ -1200,11 +1225,15 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
         p.out = static_cast<__nv_bfloat16*>(out) + done * out_stride;
         p.slots = slots + done;
         p.seq_lens = seq_lens + done;
-        Launch split(dim3(p.ctas), dim3(kvcache::SPLIT_THREADS), smem, stream, pdl);
+        Launch split(dim3(ctas), dim3(kvcache::SPLIT_THREADS), smem, stream, pdl);
         e = cudaLaunchKernelEx(&split.cfg, kernels[wide][mode], p);
         if (e == cudaSuccess) {
-            Launch join(dim3(p.seqs, c->kv_heads * p.row_tiles), dim3(kvcache::D), 0, stream, pdl);
-            e = cudaLaunchKernelEx(&join.cfg, kvcache::attention_join_kernel,
+            const int rows = std::min(p.group, wide ? 16 : 8);
+            const bool few = p.seqs * c->kv_heads * p.row_tiles <= p.workers / 4;
+            Launch join(dim3(p.seqs, c->kv_heads * p.row_tiles, rows), dim3(few ? 512 : 128), 0,
+                        stream, pdl);
+            e = cudaLaunchKernelEx(&join.cfg, few ? kvcache::attention_join_kernel<512>
+                                                  : kvcache::attention_join_kernel<128>,
                                    static_cast<const kvcache::AttentionParams>(p), wide ? 16 : 8);
         }
         if (e != cudaSuccess)
