@@ -252,19 +252,20 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 // A block is two contiguous 8 KiB tiles (K, V transposed), which each warp has
 // copied into a ring of its own in shared memory (cp.async.bulk), across the
 // borders of sequences.  From there mma.sync (m16n8k16, f16, FP32 accumulation)
-// reads its operands as they lie, 16 bytes per lane and load, with nothing
-// shuffled:
-//   * e4m3 becomes f16 exactly.  The order of a product's summation index is
-//     free as long as both operands agree, so lane (g, t) = (lane / 4, lane % 4)
-//     takes 16 consecutive dims of a K row, and the matching dims of q.
+// reads them as they lie, 16 bytes per lane and load, with nothing shuffled:
+//   * The order of a product's summation index is free as long as both operands
+//     agree, so lane (g, t) = (lane / 4, lane % 4) takes 16 consecutive dims of
+//     a K row, and the matching dims of q.
 //   * Scores come out as rows = query heads, columns = tokens; with K row
 //     16 (n / 2) + 2 j + n % 2 as column n of score tile j, lane (g, t) ends up
 //     with row g's scores of tokens 16 t .. 16 t + 15, and these are what the
 //     second product needs from it next to 16 bytes of a row of V transposed.
+//   * e4m3 becomes f16 exactly.  (mma.sync with e4m3 operands, q and the weights
+//     as sums of two e4m3, took more instructions per block, 1370 against 1080.)
 //   * q is scaled by a power of two per row, so that f16 holds it; weights are
 //     f16 in [0, 1]; block scales are applied in FP32.
 // tcgen05 would pad 4 to 16 rows to 128; here the tensor work is far below the
-// time of the loads.
+// time of the loads, and the instructions per block are what has to stay low.
 //
 // The unfinished block is BF16 and takes the same route with BF16 products, its
 // weights as a sum of two BF16 so that they keep 16 bits.
@@ -323,29 +324,31 @@ struct SplitSmem {
 };
 static_assert(2 * (sizeof(SplitSmem) + 1024) <= 228 * 1024, "two CTAs per SM");
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                        uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                         uint32_t b1) {
+struct Words {
+    uint32_t a[4];
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const Words& w, uint32_t b0, uint32_t b1) {
+    const uint32_t* a = w.a;
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
                  "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two e4m3 bytes (the low or high half of w) -> two f16.
-template <int kHalf>
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, %2;\n\t}" : "=r"(r) : "r"(w), "h"(static_cast<uint16_t>(w >> (16 * kHalf))));
-    return r;
+// Four e4m3 bytes -> two pairs of f16.
+__device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
 }
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -414,8 +417,8 @@ struct Score {
 };
 
 // One block's scores s[h][j][c] (token 16 t + 2 j + c of the block, already in
-// log2 units, -inf where not seen) -> weights in place; returns the factor of
-// what was summed before.
+// log2 units, -inf where not seen) -> weights in place, and the factor of what
+// was summed before.
 template <bool kWide>
 __device__ __forceinline__ void softmax_step(Rows<kWide>& r, float (&s)[Rows<kWide>::H][8][2],
                                              float (&old)[Rows<kWide>::H]) {
@@ -456,16 +459,19 @@ __device__ __forceinline__ int last_at_or_before(const int32_t* x, int n, int v)
 struct Walk {
     int at, end;                       // items not entered yet
     int i, pair, b0, b1, nb;           // the current pair, its blocks here [b0, b1) of nb
+    int head, row0;                    // the pair's K/V head and first query head of its group
     int slot, len, b;                  // b: the current block
     int id;                            // lane k: cache block of the k-th of 32 blocks
 
-    __device__ bool enter(const SplitSmem& sm, int pairs) {
+    __device__ bool enter(const SplitSmem& sm, int row_tiles) {
         if (at >= end) return false;
         while (sm.first[i + 1] <= at) ++i;
         slot = sm.slot[i];
         len = sm.len[i];
         nb = (len + BLOCK - 1) / BLOCK;
         pair = (at - sm.first[i]) / nb;
+        head = row_tiles == 1 ? pair : pair / row_tiles;
+        row0 = (pair - head * row_tiles) * 16;
         b = b0 = at - sm.first[i] - pair * nb;
         b1 = min(nb, b0 + end - at);
         at += b1 - b0;
@@ -609,13 +615,12 @@ attention_split_kernel(const AttentionParams p) {
     int sub = 0, fed = 0;              // part of the current block; the stage to fill next
     const auto request = [&]() {
         while (true) {
-            if (!feeding && !feed.enter(sm, pairs)) return;
+            if (!feeding && !feed.enter(sm, p.row_tiles)) return;
             feeding = true;
             if (feed.b >= feed.b1) {
                 feeding = false;
                 continue;
             }
-            const int head = feed.pair / p.row_tiles;
             const uint8_t* src;
             const float* scale = nullptr;
             int bytes = TILE_BYTES, parts = 2;
@@ -625,18 +630,18 @@ attention_split_kernel(const AttentionParams p) {
                     ++feed.b;
                     continue;
                 }
-                const int64_t block = static_cast<int64_t>(id) * p.kv_heads + head;
+                const int64_t block = static_cast<int64_t>(id) * p.kv_heads + feed.head;
                 src = (sub ? p.v_blocks : p.k_blocks) + block * TILE_BYTES;
                 scale = (sub ? p.v_scales : p.k_scales) + block;
             } else {
                 const int left = feed.len % BLOCK;
                 const int halves = left > 32 ? 2 : 1;
                 parts = 2 * halves;
-                const int half = sub % halves;
+                const int part = sub % halves;
                 src = reinterpret_cast<const uint8_t*>(sub < halves ? p.k_tail : p.v_tail) +
-                      (static_cast<int64_t>(feed.slot) * p.kv_heads + head) * (2 * TILE_BYTES) +
-                      half * TILE_BYTES;
-                bytes = min(left - 32 * half, 32) * D * 2;
+                      (static_cast<int64_t>(feed.slot) * p.kv_heads + feed.head) * (2 * TILE_BYTES) +
+                      part * TILE_BYTES;
+                bytes = min(left - 32 * part, 32) * D * 2;
             }
             if (lane == 0) {
                 const uint32_t bar = smem_u32(&sm.full[warp][fed]);
@@ -655,9 +660,6 @@ attention_split_kernel(const AttentionParams p) {
             return;
         }
     };
-    __syncwarp();
-    for (int s = 0; s < STAGES; ++s) request();
-
     int stage = 0;                     // the next stage to read
     uint32_t phase = 0;
     bool alive = true;                 // no wait has given up
@@ -674,223 +676,246 @@ attention_split_kernel(const AttentionParams p) {
                     alive = false;
                 }
         }
-        return sm.ring[warp][slot];
+        return static_cast<const uint8_t*>(sm.ring[warp][slot]);
     };
-    // The warp has read its oldest stage: fill it again.
-    const auto release = [&]() {
+
+    // One round per half block: first K (scores and weights), then V (output).
+    // A single loop, so that there is one copy of everything: unrolled code that
+    // does not fit the instruction caches was what held short sequences up.
+    int todo = STAGES;                 // stages to request: those just read
+    int half = 0;
+    bool open = false;
+    int rows = 0;
+    const __nv_bfloat16* q = nullptr;
+    uint32_t qf[H][16];                // f16, times 2^-e
+    Score<kMode> score[H];
+    Rows<kWide> r;
+    float s[H][8][2], old[H];
+    const float raw = kMode & 1 ? 2.f * LOG2E * p.scale / p.softcap : p.scale * LOG2E;
+    // Lane's dims of row g + 8 h: word pair y of chunk c covers dims 64 c + 16 t + 4 y .. + 3.
+    const auto load_q = [&](int h, int c) {
+        return g + 8 * h < rows ? *reinterpret_cast<const uint4*>(
+                                      q + (g + 8 * h) * D + 64 * (c >> 1) + 16 * t + 8 * (c & 1))
+                                : make_uint4(0, 0, 0, 0);
+    };
+    while (true) {
+        uint4 raw_q[H][4];
+        const bool fresh = !open;
+        if (fresh) {
+            if (!walk.enter(sm, p.row_tiles)) break;
+            open = true;
+            q = p.q + walk.i * p.q_stride + (walk.head * p.group + walk.row0) * D;
+            rows = min(p.group - walk.row0, ROWS);
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) raw_q[h][c] = load_q(h, c);
+                score[h].slope =
+                    (kMode & 2) && g + 8 * h < rows
+                        ? __ldg(p.alibi_slopes + walk.head * p.group + walk.row0 + g + 8 * h) * LOG2E
+                        : 0.f;
+            }
+        }
         __syncwarp();
-        if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
-        }
-        request();
-    };
-
-    while (walk.enter(sm, pairs)) {
-        const int head = walk.pair / p.row_tiles;
-        const int row0 = walk.pair % p.row_tiles * 16; // first row (query head of the group)
-        const __nv_bfloat16* q = p.q + walk.i * p.q_stride + (head * p.group + row0) * D;
-        const int rows = min(p.group - row0, ROWS);
-        const int len = walk.len;
-
-        // q fragments: k step (c, s) covers dims 64 c + 16 t + 4 s .. + 3 of lane (g, t).
-        uint4 qb[H][4];                                // as it is, BF16
-        uint32_t qf[H][16];                            // f16, times 2^-e
-        Score<kMode> score[H];
-        const float raw = kMode & 1 ? 2.f * LOG2E * p.scale / p.softcap : p.scale * LOG2E;
+#pragma unroll 1
+        for (; todo > 0; --todo) request();
+        if (fresh) {
+            r.clear();
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            const int row = g + 8 * h;
-            const bool there = row < rows;
+            for (int h = 0; h < H; ++h) {
+                const uint32_t* w = &raw_q[h][0].x;
+                float top = 0.f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                qb[h][c] = there ? *reinterpret_cast<const uint4*>(
-                                       q + row * D + 64 * (c >> 1) + 16 * t + 8 * (c & 1))
-                                 : make_uint4(0, 0, 0, 0);
-            const uint32_t* w = &qb[h][0].x;
-            float top = 0.f;
+                for (int k = 0; k < 16; ++k)
+                    top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[k])), fabsf(bf16_hi(w[k]))));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // q = (q 2^-e) 2^e with the row's largest value in [1, 2).
+                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+                const float down = __int_as_float((127 - e) << 23);
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-                top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[k])), fabsf(bf16_hi(w[k]))));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // q = (q 2^-e) 2^e with the row's largest value in [1, 2).
-            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
-            const float down = __int_as_float((127 - e) << 23);
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-                qf[h][k] = pack_f16x2(bf16_lo(w[k]) * down, bf16_hi(w[k]) * down);
-            score[h].factor = raw * __int_as_float((127 + e) << 23);
-            score[h].cap_out = p.softcap * LOG2E;
-            score[h].slope = (kMode & 2) && there
-                                 ? __ldg(p.alibi_slopes + head * p.group + row0 + row) * LOG2E
-                                 : 0.f;
+                for (int k = 0; k < 16; ++k)
+                    qf[h][k] = pack_f16x2(bf16_lo(w[k]) * down, bf16_hi(w[k]) * down);
+                score[h].factor = raw * __int_as_float((127 + e) << 23);
+                score[h].cap_out = p.softcap * LOG2E;
+            }
         }
 
-        Rows<kWide> r;
-        r.clear();
-        for (; walk.b < walk.b1; ++walk.b) {
-            float s[H][8][2], old[H];
-            if (walk.is_full()) {
-                if (walk.lookup(p, lane) < 0) {
-                    report_status(p.status, FU_DEV_CACHE_RANGE, W_ATTENTION);
-                    continue;
-                }
-                const uint8_t* tile = await(0);
+        if (walk.is_full()) {
+            if (half == 0 && walk.lookup(p, lane) < 0) {
+                report_status(p.status, FU_DEV_CACHE_RANGE, W_ATTENTION);
+                half = 1;                              // not seen: neither K nor V is here
+            } else if (half == 0) {
+                const uint8_t* tile = await(0) + (16 * (g >> 1) + (g & 1)) * D + 16 * t;
                 const float ks = sm.scale[warp][stage];
+                // Four score tiles at a time: their chains of products overlap.
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint8_t* row = tile + (16 * (g >> 1) + 2 * j + (g & 1)) * D + 16 * t;
-                    const uint4 x[2] = {*reinterpret_cast<const uint4*>(row),
-                                        *reinterpret_cast<const uint4*>(row + 64)};
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int j0 = 0; j0 < 8; j0 += 4) {
+                    float acc[4][4] = {};
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t w = (&x[k >> 2].x)[k & 3];
-                        const uint32_t a[4] = {qf[0][2 * k], kWide ? qf[H - 1][2 * k] : 0u,
-                                               qf[0][2 * k + 1],
-                                               kWide ? qf[H - 1][2 * k + 1] : 0u};
-                        mma_f16(acc, a, e4m3x2_to_f16x2<0>(w), e4m3x2_to_f16x2<1>(w));
+                    for (int y = 0; y < 2; ++y) {
+                        uint4 x[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            x[j] = *reinterpret_cast<const uint4*>(tile + 2 * (j0 + j) * D + 64 * y);
+#pragma unroll
+                        for (int k = 4 * y; k < 4 * y + 4; ++k)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t b0, b1;
+                                e4m3x4_to_f16x4((&x[j].x)[k & 3], b0, b1);
+                                mma_f16(acc[j], qf[0][2 * k], kWide ? qf[H - 1][2 * k] : 0u,
+                                        qf[0][2 * k + 1], kWide ? qf[H - 1][2 * k + 1] : 0u, b0,
+                                        b1);
+                            }
                     }
 #pragma unroll
-                    for (int h = 0; h < H; ++h)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c)
-                            s[h][j][c] = score[h](
-                                acc[2 * h + c], ks,
-                                len - 1 - (walk.b * BLOCK + 16 * t + 2 * j + c));
+                        for (int h = 0; h < H; ++h)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                s[h][j0 + j][c] = score[h](
+                                    acc[j][2 * h + c], ks,
+                                    walk.len - 1 - (walk.b * BLOCK + 16 * t + 2 * (j0 + j) + c));
                 }
-                release();
+                todo = 1;
                 softmax_step<kWide>(r, s, old);
-                uint32_t pf[4][4];                     // weights of tokens 16 t + 4 k .. + 3
+            } else {
+                uint32_t pf[H][8];                     // weights of tokens 16 t + 2 k, + 1
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        pf[k][2 * x] = pack_f16x2(s[0][2 * k + x][0], s[0][2 * k + x][1]);
-                        pf[k][2 * x + 1] =
-                            kWide ? pack_f16x2(s[H - 1][2 * k + x][0], s[H - 1][2 * k + x][1]) : 0u;
-                    }
-                tile = await(0);
+                    for (int k = 0; k < 8; ++k) pf[h][k] = pack_f16x2(s[h][k][0], s[h][k][1]);
+                const uint8_t* tile = await(0) + 16 * g * BLOCK + 16 * t;
                 const float vs = sm.scale[warp][stage];
 #pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                    const uint4 x =
-                        *reinterpret_cast<const uint4*>(tile + (16 * g + d) * BLOCK + 16 * t);
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int d0 = 0; d0 < 16; d0 += 4) {
+                    uint4 x[4];
+                    float acc[4][4] = {};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t w = (&x.x)[k];
-                        mma_f16(acc, pf[k], e4m3x2_to_f16x2<0>(w), e4m3x2_to_f16x2<1>(w));
-                    }
+                    for (int d = 0; d < 4; ++d)
+                        x[d] = *reinterpret_cast<const uint4*>(tile + (d0 + d) * BLOCK);
 #pragma unroll
-                    for (int h = 0; h < H; ++h)
+                    for (int k = 0; k < 4; ++k)
 #pragma unroll
-                        for (int c = 0; c < 2; ++c)
-                            r.o[h][d][c] = fmaf(acc[2 * h + c], vs, r.o[h][d][c] * old[h]);
+                        for (int d = 0; d < 4; ++d) {
+                            uint32_t b0, b1;
+                            e4m3x4_to_f16x4((&x[d].x)[k], b0, b1);
+                            mma_f16(acc[d], pf[0][2 * k], kWide ? pf[H - 1][2 * k] : 0u,
+                                    pf[0][2 * k + 1], kWide ? pf[H - 1][2 * k + 1] : 0u, b0, b1);
+                        }
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c)
+                                r.o[h][d0 + d][c] =
+                                    fmaf(acc[d][2 * h + c], vs, r.o[h][d0 + d][c] * old[h]);
                 }
-                release();
-                continue;
+                todo = 1;
             }
-
+        } else {
             // The unfinished block; rows behind its last token are not read.
-            const int left = len % BLOCK;
+            const int left = walk.len % BLOCK;
             const bool both = left > 32;
             const uint8_t* tile = await(0);
             const uint8_t* tile2 = both ? await(1) : tile;
-            const uint8_t* half = g < 4 ? tile : tile2 - TILE_BYTES;   // K rows from 32 on
+            if (half == 0) {
+                tile = g < 4 ? tile : tile2 - TILE_BYTES;             // rows from 32 on
+                uint4 qb[H][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int row = 16 * (g >> 1) + 2 * j + (g & 1);
-                uint4 x[4];
+                for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    x[c] = row < left ? *reinterpret_cast<const uint4*>(
-                                            half + (row * D + 64 * (c >> 1) + 16 * t +
-                                                    8 * (c & 1)) * 2)
-                                      : make_uint4(0, 0, 0, 0);
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int c = 0; c < 4; ++c) qb[h][c] = load_q(h, c);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t* w = &x[k >> 1].x + 2 * (k & 1);
-                    const uint32_t* q0 = &qb[0][k >> 1].x + 2 * (k & 1);
-                    const uint32_t* q1 = &qb[H - 1][k >> 1].x + 2 * (k & 1);
-                    const uint32_t a[4] = {q0[0], kWide ? q1[0] : 0u, q0[1], kWide ? q1[1] : 0u};
-                    mma_bf16(acc, a, w[0], w[1]);
-                }
+                for (int j = 0; j < 8; ++j) {
+                    const int row = 16 * (g >> 1) + 2 * j + (g & 1);
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    Score<kMode> plain = score[h];
-                    plain.factor = raw;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int token = 16 * t + 2 * j + c;
-                        const float x2 = plain(acc[2 * h + c], 1.f, left - 1 - token);
-                        s[h][j][c] = token < left ? x2 : -INFINITY;
+                    for (int c = 0; c < 4; ++c) {
+                        const uint4 x = row < left
+                                            ? *reinterpret_cast<const uint4*>(
+                                                  tile + (row * D + 64 * (c >> 1) + 16 * t +
+                                                          8 * (c & 1)) * 2)
+                                            : make_uint4(0, 0, 0, 0);
+                        const uint4 q0 = qb[0][c], q1 = qb[H - 1][c];
+                        mma_bf16(acc, Words{{q0.x, kWide ? q1.x : 0u, q0.y, kWide ? q1.y : 0u}}, x.x, x.y);
+                        mma_bf16(acc, Words{{q0.z, kWide ? q1.z : 0u, q0.w, kWide ? q1.w : 0u}}, x.z, x.w);
                     }
-                }
-            }
-            release();
-            if (both) release();
-            softmax_step<kWide>(r, s, old);
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                    r.o[h][d][0] *= old[h];
-                    r.o[h][d][1] *= old[h];
-                }
-            tile = await(0);
-            tile2 = both ? await(1) : tile;
-            half = t < 2 ? tile : tile2 - TILE_BYTES;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                uint4 x[4][2];                         // four tokens, dims 16 g .. 16 g + 15
-#pragma unroll
-                for (int y = 0; y < 4; ++y)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int row = 16 * t + 4 * k + y;
-                        x[y][c] = row < left ? *reinterpret_cast<const uint4*>(
-                                                   half + (row * D + 16 * g + 8 * c) * 2)
-                                             : make_uint4(0, 0, 0, 0);
-                    }
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h >= H) {
-                            hi[2 * y + h] = lo[2 * y + h] = 0u;
-                            continue;
-                        }
-                        const float w0 = s[h % H][2 * k + y][0], w1 = s[h % H][2 * k + y][1];
-                        const uint32_t top = pack_bf16x2(w0, w1);
-                        hi[2 * y + h] = top;
-                        lo[2 * y + h] = pack_bf16x2(w0 - bf16_lo(top), w1 - bf16_hi(top));
-                    }
-#pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                    const uint32_t sel = d & 1 ? 0x7632 : 0x5410;
-                    const uint32_t w0 = (&x[0][d >> 3].x)[(d & 7) >> 1];
-                    const uint32_t w1 = (&x[1][d >> 3].x)[(d & 7) >> 1];
-                    const uint32_t w2 = (&x[2][d >> 3].x)[(d & 7) >> 1];
-                    const uint32_t w3 = (&x[3][d >> 3].x)[(d & 7) >> 1];
-                    const uint32_t f0 = __byte_perm(w0, w1, sel), f1 = __byte_perm(w2, w3, sel);
-                    float acc[4] = {r.o[0][d][0], r.o[0][d][1], r.o[H - 1][d][0],
-                                    r.o[H - 1][d][1]};
-                    mma_bf16(acc, hi, f0, f1);
-                    mma_bf16(acc, lo, f0, f1);
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
-                        r.o[h][d][0] = acc[2 * h];
-                        r.o[h][d][1] = acc[2 * h + 1];
+                        Score<kMode> plain = score[h];
+                        plain.factor = raw;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int token = 16 * t + 2 * j + c;
+                            const float x = plain(acc[2 * h + c], 1.f, left - 1 - token);
+                            s[h][j][c] = token < left ? x : -INFINITY;
+                        }
+                    }
+                }
+                softmax_step<kWide>(r, s, old);
+            } else {
+                tile = t < 2 ? tile : tile2 - TILE_BYTES;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint4 x[4][2];                     // four tokens, dims 16 g .. 16 g + 15
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int row = 16 * t + 4 * k + y;
+                            x[y][c] = row < left ? *reinterpret_cast<const uint4*>(
+                                                       tile + (row * D + 16 * g + 8 * c) * 2)
+                                                 : make_uint4(0, 0, 0, 0);
+                        }
+                    uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            const float w0 = s[h][2 * k + y][0], w1 = s[h][2 * k + y][1];
+                            const uint32_t top = pack_bf16x2(w0, w1);
+                            hi[2 * y + h] = top;
+                            lo[2 * y + h] = pack_bf16x2(w0 - bf16_lo(top), w1 - bf16_hi(top));
+                        }
+#pragma unroll
+                    for (int d = 0; d < 16; ++d) {
+                        const uint32_t sel = d & 1 ? 0x7632 : 0x5410;
+                        const uint32_t w0 = (&x[0][d >> 3].x)[(d & 7) >> 1];
+                        const uint32_t w1 = (&x[1][d >> 3].x)[(d & 7) >> 1];
+                        const uint32_t w2 = (&x[2][d >> 3].x)[(d & 7) >> 1];
+                        const uint32_t w3 = (&x[3][d >> 3].x)[(d & 7) >> 1];
+                        const uint32_t f0 = __byte_perm(w0, w1, sel), f1 = __byte_perm(w2, w3, sel);
+                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            acc[2 * h] = k ? r.o[h][d][0] : r.o[h][d][0] * old[h];
+                            acc[2 * h + 1] = k ? r.o[h][d][1] : r.o[h][d][1] * old[h];
+                        }
+                        mma_bf16(acc, Words{{hi[0], hi[1], hi[2], hi[3]}}, f0, f1);
+                        mma_bf16(acc, Words{{lo[0], lo[1], lo[2], lo[3]}}, f0, f1);
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            r.o[h][d][0] = acc[2 * h];
+                            r.o[h][d][1] = acc[2 * h + 1];
+                        }
                     }
                 }
             }
-            release();
-            if (both) release();
+            todo = both ? 2 : 1;
         }
+        stage += todo;
+        if (stage >= STAGES) {
+            stage -= STAGES;
+            phase ^= 1;
+        }
+        half ^= 1;
+        if (half == 1) continue;
+        if (++walk.b < walk.b1) continue;
+        open = false;
 
         const bool whole = walk.b1 - walk.b0 == walk.nb;
         // A warp has at most two pairs that it shares with others: the one it
@@ -898,6 +923,8 @@ attention_split_kernel(const AttentionParams p) {
         const bool at_begin = walk.at - (walk.b1 - walk.b0) == begin;
         float* part =
             p.partial + (static_cast<int64_t>(worker) * 2 + (at_begin ? 0 : 1)) * ROWS * PART;
+        const int64_t out0 =
+            walk.i * p.out_stride + (walk.head * p.group + walk.row0) * D;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const int row = g + 8 * h;
@@ -907,8 +934,7 @@ attention_split_kernel(const AttentionParams p) {
             if (row >= rows) continue;
             if (whole) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                __nv_bfloat16* out = p.out + walk.i * p.out_stride +
-                                     (head * p.group + row0 + row) * D + 32 * t;
+                __nv_bfloat16* out = p.out + out0 + row * D + 32 * t;
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
