@@ -431,35 +431,28 @@ class OprojOp:
             self.handle = None
 
 
-def attention_forward(device, q_heads, kv_heads, causal, tokens, q, k, v, out, q_stride, k_stride,
-                      v_stride, out_stride, cu_seqlens, prefix_lens, alibi_slopes, docs, scale,
-                      softcap, status, status_host, timeout_ns, flags, stream):
-    """``fu_attention_forward`` on raw device pointers."""
-    if _fast is not None:
-        _fast.attention(device, q_heads, kv_heads, causal, tokens, q, k, v, out, q_stride,
-                        k_stride, v_stride, out_stride, cu_seqlens, prefix_lens, alibi_slopes,
-                        docs, scale, softcap, status, status_host, timeout_ns, flags, stream)
-        return
+def _attention_forward(device, q_heads, kv_heads, causal, tokens, q, k, v, out, q_stride, k_stride,
+                       v_stride, out_stride, cu_seqlens, prefix_lens, alibi_slopes, docs, scale,
+                       softcap, status, status_host, timeout_ns, flags, stream):
     a = AttentionArgs(device, q_heads, kv_heads, causal, tokens, q, k, v, out, q_stride, k_stride,
                       v_stride, out_stride, cu_seqlens, prefix_lens, alibi_slopes, docs, scale,
                       softcap, 0, status, status_host, timeout_ns)
     check(lib.fu_attention_forward(ctypes.byref(a), flags, stream), "fu_attention_forward")
 
 
-def kvcache_append(*args):
-    """``fu_kvcache_append`` on raw device pointers (the header's arguments)."""
-    if _fast is not None:
-        _fast.kvcache_append(*args)
-        return
+def _kvcache_append(*args):
     check(lib.fu_kvcache_append(*args), "fu_kvcache_append")
 
 
-def kvcache_attention(*args):
-    """``fu_kvcache_attention`` on raw device pointers (the header's arguments)."""
-    if _fast is not None:
-        _fast.kvcache_attention(*args)
-        return
+def _kvcache_attention(*args):
     check(lib.fu_kvcache_attention(*args), "fu_kvcache_attention")
+
+
+# The calls of the C entry points of these names with raw device pointers, in
+# the order of the header's arguments (of fu_attention_args' fields).
+attention_forward = _attention_forward if _fast is None else _fast.attention
+kvcache_append = _kvcache_append if _fast is None else _fast.kvcache_append
+kvcache_attention = _kvcache_attention if _fast is None else _fast.kvcache_attention
 
 
 def kvcache_attention_workspace(device, q_heads, kv_heads, seqs):

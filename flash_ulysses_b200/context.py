@@ -31,6 +31,7 @@ projection.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -38,6 +39,48 @@ import torch.distributed as dist
 
 from . import _C
 from .kv_cache import KvCache
+
+
+def _rows(name, t, rows, width, index):
+    """(address, row stride) of a BF16 [rows, width] tensor; raises on any other."""
+    if t.dtype is not torch.bfloat16 or t.shape != (rows, width) or t.get_device() != index:
+        raise ValueError(f"{name} must be a BF16 tensor of shape {(rows, width)} on the "
+                         f"context's device")
+    row, column = t.stride()
+    if rows == 1:
+        row = width
+    ptr = t.data_ptr()
+    if column != 1 or row < width or row % 8 or ptr % 16:
+        raise ValueError(f"{name} must be 16-byte aligned with contiguous rows whose stride is a "
+                         "multiple of 8 elements")
+    return ptr, row
+
+
+def _vector(name, t, dtype, length, index):
+    """Address of a contiguous vector of `length` elements; raises on any other."""
+    if (t.dtype is not dtype or t.shape != (length,) or not t.is_contiguous()
+            or t.get_device() != index):
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of {length} elements on "
+                         "the context's device")
+    return t.data_ptr()
+
+
+def _like_rows(t, stride, width):
+    """A new contiguous tensor of t's shape."""
+    if stride == width:
+        return torch.empty_like(t)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _no_overlap(rows, out, out_stride, out_width, t, stride, width):
+    if rows and (out < t + 2 * ((rows - 1) * stride + width)
+                 and t < out + 2 * ((rows - 1) * out_stride + out_width)):
+        raise ValueError("out must not overlap an input")
+
+
+def _check_cache(cache, kv_width, device):
+    if (cache.device is not device and cache.device != device) or cache.kv_heads * _C.FU_HEAD_DIM != kv_width:
+        raise ValueError(f"the cache must hold {kv_width // _C.FU_HEAD_DIM} K/V heads on {device}")
 
 
 class FlashUlyssesContext:
@@ -300,28 +343,20 @@ class FlashUlyssesContext:
         return out
 
     # ------------------------------------------------------------ attention
-    def _row_stride(self, name, t, rows, heads):
-        """Row stride of a BF16 [rows, heads * 128] tensor; raises on any other."""
-        width = heads * self.head_dim
-        if (t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows
-                or t.shape[1] != width or t.device != self.device):
-            raise ValueError(f"{name} must be a BF16 tensor of shape {(rows, width)} "
-                             f"on {self.device}")
-        row, column = t.stride()
-        if rows == 1:
-            row = width
-        if column != 1 or row < width or row % 8 or t.data_ptr() % 16:
-            raise ValueError(f"{name} must be 16-byte aligned with contiguous rows whose stride "
-                             "is a multiple of 8 elements")
-        return row
+    # These calls are a few microseconds on the GPU at decode sizes, so their
+    # checks ask each tensor only once for what they need.
+    @functools.cached_property
+    def _widths(self):
+        """Columns of Q and of K/V rows, and the device index (-1: the CPU)."""
+        index = self.device.index
+        return (self.output_q_heads * self.head_dim, self.output_kv_heads * self.head_dim,
+                -1 if index is None else index)
 
-    def _vector(self, name, t, dtype, length):
-        """Address of a contiguous vector of `length` elements; raises on any other."""
-        if (t.dtype != dtype or t.dim() != 1 or t.shape[0] != length or not t.is_contiguous()
-                or t.device != self.device):
-            raise ValueError(f"{name} must be a contiguous {dtype} vector of {length} elements "
-                             f"on {self.device}")
-        return t.data_ptr()
+    @functools.cached_property
+    def _attention_scratch(self):
+        """Bytes of the decode attention's scratch."""
+        return _C.kvcache_attention_workspace(self._widths[2], self.output_q_heads,
+                                              self.output_kv_heads, 1)
 
     def _score_options(self, scale, softcap, alibi_slopes):
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
@@ -330,32 +365,15 @@ class FlashUlyssesContext:
             raise ValueError("scale must be finite, softcap finite and not negative")
         slopes = None
         if alibi_slopes is not None:
-            slopes = self._vector("alibi_slopes", alibi_slopes, torch.float32,
-                                  self.output_q_heads)
+            slopes = _vector("alibi_slopes", alibi_slopes, torch.float32, self.output_q_heads,
+                             self._widths[2])
         return scale, softcap, slopes
-
-    def _output(self, out, rows, *inputs):
-        """`out` or a new tensor, and its row stride."""
-        heads = self.output_q_heads
-        if out is None:
-            out = torch.empty(rows, heads * self.head_dim, dtype=torch.bfloat16,
-                              device=self.device)
-            return out, heads * self.head_dim
-        stride = self._row_stride("out", out, rows, heads)
-        begin, end = out.data_ptr(), out.data_ptr() + 2 * ((rows - 1) * stride + out.shape[1])
-        for t in inputs:
-            first = t.data_ptr()
-            last = first + 2 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])
-            if rows and begin < last and first < end:
-                raise ValueError("out must not overlap an input")
-        return out, stride
 
     def _raise_earlier(self):
         if self._status.value:
             raise RuntimeError("an earlier call failed on the device: "
                                + _C.decode_status(self._status.value))
 
-    @torch.no_grad()
     def ulysses_attention_forward(self, q, k, v, *, cu_seqlens=None, prefix_lens=None,
                                   causal=True, scale=None, softcap=0.0, alibi_slopes=None,
                                   out=None):
@@ -387,28 +405,35 @@ class FlashUlyssesContext:
         with other lengths in the same tensors.
         """
         rows = q.shape[0]
-        strides = (self._row_stride("q", q, rows, self.output_q_heads),
-                   self._row_stride("k", k, rows, self.output_kv_heads),
-                   self._row_stride("v", v, rows, self.output_kv_heads))
+        q_width, kv_width, index = self._widths
+        q_ptr, q_stride = _rows("q", q, rows, q_width, index)
+        k_ptr, k_stride = _rows("k", k, rows, kv_width, index)
+        v_ptr, v_stride = _rows("v", v, rows, kv_width, index)
         if rows > 1 << 30:
             raise ValueError("at most 2^30 rows")
         scale, softcap, slopes = self._score_options(scale, softcap, alibi_slopes)
         docs, cu, prefix = 1, None, None
         if cu_seqlens is not None:
             docs = cu_seqlens.numel() - 1
-            cu = self._vector("cu_seqlens", cu_seqlens, torch.int32, max(docs + 1, 1))
+            cu = _vector("cu_seqlens", cu_seqlens, torch.int32, max(docs + 1, 1), index)
         if prefix_lens is not None:
             if not causal:
                 raise ValueError("prefix_lens needs causal=True")
-            prefix = self._vector("prefix_lens", prefix_lens, torch.int32, docs)
+            prefix = _vector("prefix_lens", prefix_lens, torch.int32, docs, index)
         self._raise_earlier()
-        out, out_stride = self._output(out, rows, q, k, v)
+        if out is None:
+            out = _like_rows(q, q_stride, q_width)
+            out_ptr, out_stride = out.data_ptr(), q_width
+        else:
+            out_ptr, out_stride = _rows("out", out, rows, q_width, index)
+            _no_overlap(rows, out_ptr, out_stride, q_width, q_ptr, q_stride, q_width)
+            _no_overlap(rows, out_ptr, out_stride, q_width, k_ptr, k_stride, kv_width)
+            _no_overlap(rows, out_ptr, out_stride, q_width, v_ptr, v_stride, kv_width)
         if rows == 0 or docs == 0:
             return out
-        index = self.device.index
-        _C.attention_forward(index, self.output_q_heads, self.output_kv_heads, int(bool(causal)),
-                             rows, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                             *strides, out_stride, cu, prefix, slopes, docs, scale, softcap,
+        _C.attention_forward(index, self.output_q_heads, self.output_kv_heads, 1 if causal else 0,
+                             rows, q_ptr, k_ptr, v_ptr, out_ptr, q_stride, k_stride, v_stride,
+                             out_stride, cu, prefix, slopes, docs, scale, softcap,
                              self._status.device_ptr, self._status.host_ptr, 0, 0,
                              _C.current_stream_handle(index))
         return out
@@ -420,12 +445,6 @@ class FlashUlyssesContext:
         return KvCache.allocate(num_blocks, max_seqs, max_blocks, self.output_kv_heads,
                                 self.device)
 
-    def _check_cache(self, cache):
-        if cache.device != self.device or cache.kv_heads != self.output_kv_heads:
-            raise ValueError(f"the cache must hold {self.output_kv_heads} K/V heads "
-                             f"on {self.device}")
-
-    @torch.no_grad()
     def kv_cache_append(self, cache, k, v, slots, seq_lens, *, cu_seqlens=None):
         """Write new K/V rows into ``cache`` (no counterpart in the reference).
 
@@ -446,25 +465,25 @@ class FlashUlyssesContext:
         nothing is written for them.
         """
         rows, count = k.shape[0], slots.numel()
-        k_stride = self._row_stride("k", k, rows, self.output_kv_heads)
-        v_stride = self._row_stride("v", v, rows, self.output_kv_heads)
-        self._check_cache(cache)
+        _, kv_width, index = self._widths
+        k_ptr, k_stride = _rows("k", k, rows, kv_width, index)
+        v_ptr, v_stride = _rows("v", v, rows, kv_width, index)
+        _check_cache(cache, kv_width, self.device)
         if rows > 1 << 30 or count > 1 << 24:
             raise ValueError("at most 2^30 rows and 2^24 sequences")
-        slot_ptr = self._vector("slots", slots, torch.int32, count if cu_seqlens is not None
-                                else rows)
-        lens_ptr = self._vector("seq_lens", seq_lens, torch.int32, count)
+        slot_ptr = _vector("slots", slots, torch.int32, rows if cu_seqlens is None else count,
+                           index)
+        lens_ptr = _vector("seq_lens", seq_lens, torch.int32, count, index)
         cu = None
         if cu_seqlens is not None:
-            cu = self._vector("cu_seqlens", cu_seqlens, torch.int32, count + 1)
+            cu = _vector("cu_seqlens", cu_seqlens, torch.int32, count + 1, index)
         self._raise_earlier()
         if rows == 0 or count == 0:
             return
-        _C.kvcache_append(cache._address, k.data_ptr(), v.data_ptr(), k_stride, v_stride, rows,
-                          slot_ptr, lens_ptr, cu, count, self._status.device_ptr,
-                          self._status.host_ptr, 0, _C.current_stream_handle(self.device.index))
+        _C.kvcache_append(cache._address, k_ptr, v_ptr, k_stride, v_stride, rows, slot_ptr,
+                          lens_ptr, cu, count, self._status.device_ptr, self._status.host_ptr, 0,
+                          _C.current_stream_handle(index))
 
-    @torch.no_grad()
     def kv_cache_attention(self, cache, q, slots, seq_lens, *, scale=None, softcap=0.0,
                            alibi_slopes=None, out=None):
         """Attention of one token per sequence over ``cache`` (no counterpart
@@ -480,24 +499,28 @@ class FlashUlyssesContext:
         fit the cache are reported by the next call or ``check()``.
         """
         rows = q.shape[0]
-        q_stride = self._row_stride("q", q, rows, self.output_q_heads)
-        self._check_cache(cache)
+        q_width, kv_width, index = self._widths
+        q_ptr, q_stride = _rows("q", q, rows, q_width, index)
+        _check_cache(cache, kv_width, self.device)
         if rows > 1 << 24:
             raise ValueError("at most 2^24 sequences")
-        slot_ptr = self._vector("slots", slots, torch.int32, rows)
-        lens_ptr = self._vector("seq_lens", seq_lens, torch.int32, rows)
+        slot_ptr = _vector("slots", slots, torch.int32, rows, index)
+        lens_ptr = _vector("seq_lens", seq_lens, torch.int32, rows, index)
         scale, softcap, slopes = self._score_options(scale, softcap, alibi_slopes)
         self._raise_earlier()
-        out, out_stride = self._output(out, rows, q)
+        if out is None:
+            out = _like_rows(q, q_stride, q_width)
+            out_ptr, out_stride = out.data_ptr(), q_width
+        else:
+            out_ptr, out_stride = _rows("out", out, rows, q_width, index)
+            _no_overlap(rows, out_ptr, out_stride, q_width, q_ptr, q_stride, q_width)
         if rows == 0:
             return out
-        index = self.device.index
         # Scratch from torch's allocator, so calls on other streams and captured
         # graphs each have their own.
-        nbytes = _C.kvcache_attention_workspace(index, self.output_q_heads,
-                                                self.output_kv_heads, rows)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        _C.kvcache_attention(cache._address, q.data_ptr(), q_stride, out.data_ptr(), out_stride,
+        nbytes = self._attention_scratch
+        work = q.new_empty((nbytes + 1) // 2)
+        _C.kvcache_attention(cache._address, q_ptr, q_stride, out_ptr, out_stride,
                              self.output_q_heads, slot_ptr, lens_ptr, rows, scale, softcap,
                              slopes, work.data_ptr(), nbytes, self._status.device_ptr,
                              self._status.host_ptr, 0, _C.current_stream_handle(index))

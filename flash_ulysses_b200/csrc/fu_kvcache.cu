@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -1189,14 +1190,47 @@ extern "C" int fu_kvcache_append(const fu_kvcache* c, const void* k, const void*
     return FU_OK;
 }
 
-// CTAs of the split kernel: two per SM (its shared memory allows no more).
+typedef void (*SplitKernel)(kvcache::AttentionParams);
+static SplitKernel split_kernel(bool wide, int mode) {
+    static const SplitKernel kernels[2][4] = {
+        {kvcache::attention_split_kernel<false, 0>, kvcache::attention_split_kernel<false, 1>,
+         kvcache::attention_split_kernel<false, 2>, kvcache::attention_split_kernel<false, 3>},
+        {kvcache::attention_split_kernel<true, 0>, kvcache::attention_split_kernel<true, 1>,
+         kvcache::attention_split_kernel<true, 2>, kvcache::attention_split_kernel<true, 3>}};
+    return kernels[wide][mode];
+}
+
+// CTAs of the split kernel on a device: two per SM (its shared memory allows no
+// more).  Asked once; 0 if there is no such device.
+constexpr int MAX_DEVICES = 64;
 static int split_ctas(int device) {
-    int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
-        cudaGetLastError();
-        return 0;
+    static std::atomic<int> known[MAX_DEVICES];
+    if (device < 0 || device >= MAX_DEVICES) return 0;
+    int ctas = known[device].load(std::memory_order_relaxed);
+    if (ctas == 0) {
+        int sms = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        ctas = 2 * sms;
+        known[device].store(ctas, std::memory_order_relaxed);
     }
-    return 2 * sms;
+    return ctas;
+}
+
+// Raises the split kernels' shared-memory limit once per device (the current one).
+static cudaError_t prepare_split(int device) {
+    static std::atomic<bool> done[MAX_DEVICES];
+    if (done[device].load(std::memory_order_acquire)) return cudaSuccess;
+    for (int k = 0; k < 8; ++k) {
+        cudaError_t e = cudaFuncSetAttribute(split_kernel(k >> 2, k & 3),
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             sizeof(kvcache::SplitSmem));
+        if (e != cudaSuccess) return e;
+    }
+    done[device].store(true, std::memory_order_release);
+    return cudaSuccess;
 }
 
 extern "C" int64_t fu_kvcache_attention_workspace(int32_t device, int32_t q_heads,
@@ -1253,9 +1287,10 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
     p.plan = static_cast<kvcache::Plan*>(workspace);
     p.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + sizeof(kvcache::Plan));
     const int ctas = split_ctas(c->device);
+    if (ctas == 0) return set_error(FU_ERR_INVALID, "device %d is not available", c->device);
     p.workers = ctas * kvcache::WARPS;
-    const int64_t per_seq = static_cast<int64_t>(kvcache::pair_cost(1)) +
-                            (2ll * c->max_blocks + 1) * c->kv_heads * p.row_tiles;
+    // The longest part of the line that one sequence can take.
+    const int64_t per_seq = (2ll * c->max_blocks + 3) * c->kv_heads * p.row_tiles;
     if (per_seq > INT32_MAX)
         return set_error(FU_ERR_INVALID, "max_blocks * kv_heads is too large for one call");
     const int64_t batch = std::min<int64_t>(kvcache::MAX_BATCH, INT32_MAX / per_seq);
@@ -1265,14 +1300,8 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
     if (!guard.ok()) return set_error(FU_ERR_INVALID, "device %d is not available", c->device);
     const bool wide = p.group > 8, pdl = (flags & FU_FWD_NO_PDL) == 0;
     const int mode = (softcap > 0.f ? 1 : 0) | (alibi_slopes != nullptr ? 2 : 0);
-    void (*const kernels[2][4])(kvcache::AttentionParams) = {
-        {kvcache::attention_split_kernel<false, 0>, kvcache::attention_split_kernel<false, 1>,
-         kvcache::attention_split_kernel<false, 2>, kvcache::attention_split_kernel<false, 3>},
-        {kvcache::attention_split_kernel<true, 0>, kvcache::attention_split_kernel<true, 1>,
-         kvcache::attention_split_kernel<true, 2>, kvcache::attention_split_kernel<true, 3>}};
     const int smem = sizeof(kvcache::SplitSmem);
-    cudaError_t e = cudaFuncSetAttribute(kernels[wide][mode],
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = prepare_split(c->device);
     if (e != cudaSuccess)
         return set_error(FU_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     for (int64_t done = 0; done < seqs; done += batch) {
@@ -1282,7 +1311,7 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
         p.slots = slots + done;
         p.seq_lens = seq_lens + done;
         Launch split(dim3(ctas), dim3(kvcache::SPLIT_THREADS), smem, stream, pdl);
-        e = cudaLaunchKernelEx(&split.cfg, kernels[wide][mode], p);
+        e = cudaLaunchKernelEx(&split.cfg, split_kernel(wide, mode), p);
         if (e == cudaSuccess) {
             const int rows = std::min(p.group, wide ? 16 : 8);
             const bool few = p.seqs * c->kv_heads * p.row_tiles <= p.workers / 4;
