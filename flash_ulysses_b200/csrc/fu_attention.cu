@@ -62,9 +62,9 @@ constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;   // room to align the base to 1 K
 static_assert(SMEM_ALLOC <= 232448, "exceeds the 227 KiB per-CTA shared memory limit");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TM_S = 0, TM_O = 256;        // + 128 * tile
-// Registers: 3 warpgroups launch with 168 each; the softmax takes 224, the
-// others keep 56 (224 + 224 + 56 = 3 * 168).
-constexpr int SOFTMAX_REGS = 224, OTHER_REGS = 56;
+// Registers: 3 warpgroups launch with 168 each; the softmax takes 216, the
+// others keep 72 (216 + 216 + 72 = 3 * 168).
+constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
 constexpr float LOG2E = 1.4426950408889634f;
 // Every so manieth pair of a row's weights is computed on the FMA pipes
 // (ex2_poly), the others by the special-function unit, whose 16 results per
@@ -128,13 +128,9 @@ __device__ __forceinline__ int2 seen_rows(const Params& p, int i) {
 // kv0 + 128 j on; query tile t takes part in the key tiles [first[t], last[t]).
 struct Work {
     int row0, head, kv0, tiles, first[2], last[2];
-    int clear_lo, clear_hi;            // keys [clear_lo, clear_hi) are seen by every valid row
-    __device__ bool active(int t, int j) const { return j >= first[t] && j < last[t]; }
+    int clear0, clear1;                // key tiles that every valid row sees all of
     // Whether some row does not see some key of tile j.
-    __device__ bool edge(int j) const {
-        const int k = kv0 + j * TILE;
-        return k < clear_lo || k + TILE > clear_hi;
-    }
+    __device__ bool edge(int j) const { return j < clear0 || j >= clear1; }
 };
 
 // `seen[t]` holds the ranges of tile t's first and last row that belongs to a
@@ -144,8 +140,8 @@ __device__ __forceinline__ Work make_work(const int2 (*seen)[2], int row0, int h
     w.row0 = row0;
     w.head = head;
     w.kv0 = seen[0][0].x;
-    w.clear_lo = seen[valid > TILE][1].x;
-    w.clear_hi = seen[0][0].y;
+    w.clear0 = (max(seen[valid > TILE][1].x - w.kv0, 0) + TILE - 1) / TILE;
+    w.clear1 = max(seen[0][0].y - w.kv0, 0) / TILE;
     w.tiles = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -171,15 +167,56 @@ __device__ __forceinline__ bool drain_wait(uint32_t bar, uint32_t parity, uint64
     return true;
 }
 
-// D[tmem] (+)= A[tmem] * B[smem], BF16 inputs, FP32 accumulate.
-__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                               uint32_t idesc, uint32_t accumulate) {
+// The MMAs' issue has to stay ahead of the tensor cores, 64 clocks an instruction,
+// in a warp that shares its scheduler with two of the softmax.  So a descriptor is
+// not put together for each (only its low word differs, the address in units of 16
+// bytes, by constants), and the whole warp runs the issuing code with the same
+// values, so that they sit in uniform registers; `one` is set in the lane that
+// issues.  (In one lane's branch each operand of each instruction had to be moved
+// there: 75 to 110 clocks an instruction.)
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);    // stride 1024, version 1, swizzle 128
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t leading_bytes) {
+    return ((saddr >> 4) & 0x3fffu) | ((leading_bytes >> 4) << 16);
+}
+
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(r));
+    return r;
+}
+
+// D[tmem] (+)= A[smem] * B[smem], BF16 inputs, FP32 accumulate.
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                       uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)),
+          "n"(DESC_HI), "r"(one)
         : "memory");
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], BF16 inputs, FP32 accumulate.
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d_tmem, uint32_t a_tmem,
+                                       uint32_t b_lo, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)),
+          "n"(DESC_HI), "r"(one)
+        : "memory");
+}
+
+// Arrive on `bar` once every tcgen05 op issued so far by lane `one` is done.
+__device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar), "r"(one) : "memory");
 }
 
 // Each thread's 32 (16) registers -> consecutive columns of its TMEM lane.
@@ -319,63 +356,74 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
     // S = Q K^T: both K-major.  O += P V: P from TMEM, V [keys, dims] MN-major.
     const uint32_t idesc_s = make_idesc_bf16_f32(TILE, TILE, false, false) | (p.negate << 13);
     constexpr uint32_t idesc_o = make_idesc_bf16_f32(TILE, D, false, true);
-    const uint32_t q = smem_u32(smem + OFF_Q), ring = smem_u32(smem + OFF_KV);
-    const auto wait = [&](uint32_t bar, uint32_t parity, int where) {
-        return fu_wait_parity(bar, parity, abort_flag, p.timeout_ns, p.status, where);
+    const uint32_t q_lo = desc_lo(smem_u32(smem + OFF_Q), 16), ring = smem_u32(smem + OFF_KV);
+    const uint32_t one = elect_one();
+    const auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        return __all_sync(0xffffffffu, fu_wait_parity(bar, parity, abort_flag, p.timeout_ns,
+                                                      p.status, where));
     };
-    uint32_t p_phase[2] = {0, 0};
+    const auto same = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+    const int first0 = same(w.first[0]), first1 = same(w.first[1]);
+    const int last0 = same(w.last[0]), last1 = same(w.last[1]);
+    const int tiles = same(w.tiles), clear0 = same(w.clear0), clear1 = same(w.clear1);
+    tmem = same(tmem);
+    uint32_t p_phase0 = 0, p_phase1 = 0;
+    // Ring stages and phases of V_j and K_(j+1), and the count of V_j.
+    int sv = STAGES - 1, sk = 0, sc = STAGES - 1;
+    uint32_t v_phase = 1, k_phase = 0, c_phase = 1;
     bool ok = wait(b.q, 0, W_Q);
     // Step j: the products P V of key tile j, each followed by the same query
     // tile's scores of key tile j + 1.
-    for (int j = -1; ok && j < w.tiles; ++j) {
-        const int iv = 2 * j + 1, ik = 2 * j + 2;       // ring positions of V_j and K_(j+1)
-        const int sv = iv % STAGES, sk = ik % STAGES;
+#pragma unroll 1
+    for (int j = -1; ok && j < tiles; ++j) {
+        const uint32_t v_lo = desc_lo(ring + sv * TILE_BYTES, BOX_BYTES);   // 64-column boxes
+        const uint32_t k_lo = desc_lo(ring + sk * TILE_BYTES, 16);
         if (j >= 0) {
-            if (w.edge(j)) {
-                ok = wait(b.clean + 8 * (j % STAGES), (j / STAGES) & 1, W_CLEAN);
-            } else {
-                ok = wait(b.kv_full + 8 * sv, (iv / STAGES) & 1, W_KV_FULL);
-            }
+            const bool edge = j < clear0 || j >= clear1;
+            ok = wait(edge ? b.clean + 8 * sc : b.kv_full + 8 * sv, edge ? c_phase : v_phase,
+                      edge ? W_CLEAN : W_KV_FULL);
             if (!ok) break;
         }
-        if (j + 1 < w.tiles && !(ok = wait(b.kv_full + 8 * sk, (ik / STAGES) & 1, W_KV_FULL))) break;
+        if (j + 1 < tiles && !(ok = wait(b.kv_full + 8 * sk, k_phase, W_KV_FULL))) break;
         tc_fence_after();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            if (!ok) break;
-            if (j >= 0 && w.active(t, j)) {
+            const int first = t ? first1 : first0, last = t ? last1 : last0;
+            uint32_t& p_phase = t ? p_phase1 : p_phase0;
+            if (j >= first && j < last) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    if (!ok || !(ok = wait(b.p + 16 * t + 8 * half, p_phase[t], W_P))) break;
+                    if (ok) ok = wait(b.p + 16 * t + 8 * half, p_phase, W_P);
+                    if (!ok) break;
                     tc_fence_after();
 #pragma unroll
                     for (int k = 4 * half; k < 4 * half + 4; ++k)
-                        tc_mma_bf16_ts(tmem + TM_O + t * TILE, tmem + TM_S + t * TILE + 8 * k,
-                                       make_smem_desc_sw128(ring + sv * TILE_BYTES + k * 16 * 128,
-                                                            BOX_BYTES, 1024),
-                                       idesc_o, j > w.first[t] || k > 0);
+                        mma_ts(one, tmem + TM_O + t * TILE, tmem + TM_S + t * TILE + 8 * k,
+                               v_lo + (k * 16 * 128 >> 4), idesc_o, k > 0 || j > first);
                 }
                 if (!ok) break;
-                p_phase[t] ^= 1;
-                if (j + 1 == w.last[t]) tc_commit(b.o + 8 * t);
+                p_phase ^= 1;
+                if (j + 1 == last) commit(one, b.o + 8 * t);
             }
-            if (j >= 0 && t == 1) tc_commit(b.kv_empty + 8 * sv);
-            if (w.active(t, j + 1)) {
+            if (t == 1 && j >= 0) commit(one, b.kv_empty + 8 * sv);
+            if (j + 1 >= first && j + 1 < last) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t at = (k / 4) * BOX_BYTES + (k % 4) * 32;
-                    tc_mma_bf16(tmem + TM_S + t * TILE,
-                                make_smem_desc_sw128(q + t * TILE_BYTES + at, 16, 1024),
-                                make_smem_desc_sw128(ring + sk * TILE_BYTES + at, 16, 1024),
-                                idesc_s, k > 0);
+                    const uint32_t at = ((k / 4) * BOX_BYTES + (k % 4) * 32) >> 4;
+                    mma_ss(one, tmem + TM_S + t * TILE, q_lo + t * (TILE_BYTES >> 4) + at,
+                           k_lo + at, idesc_s, k > 0);
                 }
-                tc_commit(b.s + 8 * t);
+                commit(one, b.s + 8 * t);
             }
-            if (j + 1 < w.tiles && t == 1) tc_commit(b.kv_empty + 8 * sk);
+            if (t == 1 && j + 1 < tiles) commit(one, b.kv_empty + 8 * sk);
         }
+        sv = sv + 2 < STAGES ? sv + 2 : (v_phase ^= 1, sv + 2 - STAGES);
+        sk = sk + 2 < STAGES ? sk + 2 : (k_phase ^= 1, sk + 2 - STAGES);
+        sc = sc + 1 < STAGES ? sc + 1 : (c_phase ^= 1, 0);
     }
-    // Every MMA this thread issued must finish before TMEM is released.
-    tc_commit(b.done);
+    // Every MMA this warp issued must finish before TMEM is released.
+    commit(one, b.done);
     drain_wait(b.done, 0, p.timeout_ns, p.status);
 }
 
@@ -712,7 +760,7 @@ attention_kernel(const __grid_constant__ Params p) {
             if (warp == 8) {
                 if ((threadIdx.x & 31) == 0) run_loads(p, w, smem, b, abort_flag);
             } else if (warp == 9) {
-                if ((threadIdx.x & 31) == 0) run_mma(p, w, smem, tmem, b, abort_flag);
+                run_mma(p, w, smem, tmem, b, abort_flag);
             } else {
                 run_clean(p, w, smem, b, abort_flag, found);
             }
