@@ -68,8 +68,9 @@ constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
 constexpr float LOG2E = 1.4426950408889634f;
 // Every so manieth pair of a row's weights is computed on the FMA pipes
 // (ex2_poly), the others by the special-function unit, whose 16 results per
-// clock and SM would otherwise take as long as the tile's matrix products.
-constexpr int POLY_EVERY = 4;
+// clock and SM take as long as the tile's matrix products.  (Every fourth or
+// none took the same time or longer; with a cap the FMA pipes are busy with it.)
+constexpr int POLY_EVERY = 8;
 
 // Status "where" codes of this kernel.
 enum : int {
@@ -372,6 +373,12 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
     // Ring stages and phases of V_j and K_(j+1), and the count of V_j.
     int sv = STAGES - 1, sk = 0, sc = STAGES - 1;
     uint32_t v_phase = 1, k_phase = 0, c_phase = 1;
+    const auto v_arrived = [&](int j) {
+        if (j < 0 || j >= tiles) return true;
+        const bool edge = j < clear0 || j >= clear1;
+        return wait(edge ? b.clean + 8 * sc : b.kv_full + 8 * sv, edge ? c_phase : v_phase,
+                    edge ? W_CLEAN : W_KV_FULL);
+    };
     bool ok = wait(b.q, 0, W_Q);
     // Step j: the products P V of key tile j, each followed by the same query
     // tile's scores of key tile j + 1.
@@ -379,18 +386,18 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
     for (int j = -1; ok && j < tiles; ++j) {
         const uint32_t v_lo = desc_lo(ring + sv * TILE_BYTES, BOX_BYTES);   // 64-column boxes
         const uint32_t k_lo = desc_lo(ring + sk * TILE_BYTES, 16);
-        if (j >= 0) {
-            const bool edge = j < clear0 || j >= clear1;
-            ok = wait(edge ? b.clean + 8 * sc : b.kv_full + 8 * sv, edge ? c_phase : v_phase,
-                      edge ? W_CLEAN : W_KV_FULL);
-            if (!ok) break;
-        }
-        if (j + 1 < tiles && !(ok = wait(b.kv_full + 8 * sk, k_phase, W_KV_FULL))) break;
-        tc_fence_after();
+        const uint32_t v_empty = b.kv_empty + 8 * sv, k_empty = b.kv_empty + 8 * sk;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int first = t ? first1 : first0, last = t ? last1 : last0;
             uint32_t& p_phase = t ? p_phase1 : p_phase0;
+            if (t == 1) {
+                // The next step's V is looked for while the first query tile's
+                // products run; K, which comes later, just before it is needed.
+                sv = sv + 2 < STAGES ? sv + 2 : (v_phase ^= 1, sv + 2 - STAGES);
+                sc = sc + 1 < STAGES ? sc + 1 : (c_phase ^= 1, 0);
+                if (!(ok = v_arrived(j + 1))) break;
+            }
             if (j >= first && j < last) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -406,8 +413,11 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
                 p_phase ^= 1;
                 if (j + 1 == last) commit(one, b.o + 8 * t);
             }
-            if (t == 1 && j >= 0) commit(one, b.kv_empty + 8 * sv);
+            if (t == 1 && j >= 0) commit(one, v_empty);
+            if (t == 0 && j + 1 < tiles && !(ok = wait(b.kv_full + 8 * sk, k_phase, W_KV_FULL)))
+                break;
             if (j + 1 >= first && j + 1 < last) {
+                tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t at = ((k / 4) * BOX_BYTES + (k % 4) * 32) >> 4;
@@ -416,11 +426,9 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
                 }
                 commit(one, b.s + 8 * t);
             }
-            if (t == 1 && j + 1 < tiles) commit(one, b.kv_empty + 8 * sk);
+            if (t == 1 && j + 1 < tiles) commit(one, k_empty);
         }
-        sv = sv + 2 < STAGES ? sv + 2 : (v_phase ^= 1, sv + 2 - STAGES);
         sk = sk + 2 < STAGES ? sk + 2 : (k_phase ^= 1, sk + 2 - STAGES);
-        sc = sc + 1 < STAGES ? sc + 1 : (c_phase ^= 1, 0);
     }
     // Every MMA this warp issued must finish before TMEM is released.
     commit(one, b.done);
@@ -580,7 +588,7 @@ __device__ void run_softmax(const Params& p, const Work& w, uint8_t* smem, uint3
             const float f = top == -INFINITY ? 1.f : ex2((m - top) * c);
             l *= f;
             m = top;
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < 4; ++k) {
                 uint32_t o[32];
                 tmem_ld_32cols(tm_o + 32 * k, o);
@@ -599,7 +607,7 @@ __device__ void run_softmax(const Params& p, const Work& w, uint8_t* smem, uint3
             for (int q = 0; q < 16; ++q) {
                 const f32x2 x = pair(s[32 * k + 2 * q], s[32 * k + 2 * q + 1]);
                 f32x2 y = kMode ? add2(x, base) : fma2(x, c2, base);
-                if (q % POLY_EVERY == POLY_EVERY - 1) {
+                if (!(kMode & 1) && q % POLY_EVERY == POLY_EVERY - 1) {
                     y = ex2_poly(y);
                 } else {
                     const float2 z = both(y);
