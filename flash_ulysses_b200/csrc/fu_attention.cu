@@ -1,8 +1,9 @@
 // Attention over the exchanged Q/K/V rows (sm_100a): packed documents, causal,
 // prefix or full masks, scores capped by a tanh and/or lowered with distance.
 //
-// A CTA computes one query head's 256 rows as two tiles of 128, and walks the
-// keys that any of its rows sees in tiles of 128 with an online softmax:
+// A CTA takes items -- one query head's 256 rows, as two tiles of 128 -- and for
+// each walks the keys that any of the rows sees in tiles of 128 with an online
+// softmax:
 //     S = Q K^T          tcgen05, Q and K from shared memory, S in TMEM
 //     m' = max(m, S), P = 2^(c S - c m'), l = l 2^(c m - c m') + sum P
 //     O = O 2^(c m - c m') + P V     tcgen05, P from TMEM, V from shared memory
@@ -13,6 +14,13 @@
 // TMA loads, warp 9 the MMA issue (and TMEM), warps 10-11 clean V tiles at the
 // edge of a mask (below).  While one tile's scores go through its softmax the
 // tensor cores work on the other tile.
+//
+// The grid has a CTA per item, but one that runs (one per SM) takes over the items of
+// CTAs that have not started, one after another.  Warp 8 works out the next one and
+// hands it to the others through a ring in shared memory, so that an item's loads
+// and first scores run under the end of the one before (a CTA per item spent 3.3 us
+// before its first scores and 1.5 us after its last product).  Items go longest
+// first; with documents their order is found by counting (Params::ranked).
 //
 // TMEM (512 columns): S0, S1, O0, O1, 128 columns each; P, two BF16 per
 // column, overwrites the first 64 columns of its tile's S.  The tile's next S
@@ -52,11 +60,14 @@ constexpr int NUM_THREADS = 384;
 constexpr int TILE_BYTES = TILE * D * 2;        // 32 KiB: two 64-column boxes
 constexpr int BOX_BYTES = TILE_BYTES / 2;
 constexpr int STAGES = 5;                       // K and V tiles in turn
+constexpr int SLOTS = 4;                        // items handed out and not finished
+constexpr int MAX_RANKED = 256;                 // row blocks that are put in order of their length
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = OFF_Q + 2 * TILE_BYTES;
-constexpr int OFF_SEEN = OFF_KV + STAGES * TILE_BYTES;      // int2[2][2]
-constexpr int OFF_BAR = OFF_SEEN + 64;
-constexpr int OFF_MISC = OFF_BAR + 8 * 32;
+constexpr int OFF_ITEM = OFF_KV + STAGES * TILE_BYTES;      // Item[SLOTS]
+constexpr int OFF_RANK = OFF_ITEM + SLOTS * 64;             // uint8_t[MAX_RANKED]
+constexpr int OFF_BAR = OFF_RANK + MAX_RANKED;
+constexpr int OFF_MISC = OFF_BAR + 8 * 40;
 constexpr int SMEM_BYTES = OFF_MISC + 64;
 constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;   // room to align the base to 1 KiB
 static_assert(SMEM_ALLOC <= 232448, "exceeds the 227 KiB per-CTA shared memory limit");
@@ -75,7 +86,7 @@ constexpr int POLY_EVERY = 8;
 // Status "where" codes of this kernel.
 enum : int {
     W_CU_SEQLENS = 64, W_Q = 65, W_KV_FULL = 66, W_KV_EMPTY = 67, W_S = 68, W_P = 69, W_O = 70,
-    W_CLEAN = 71, W_DRAIN = 72,
+    W_CLEAN = 71, W_DRAIN = 72, W_ITEM = 73, W_SLOT = 74, W_Q_EMPTY = 75,
 };
 
 struct Params {
@@ -89,16 +100,22 @@ struct Params {
     int32_t* status;
     unsigned long long timeout_ns;
     int32_t tokens, docs, q_heads, group, causal;
+    int32_t row_blocks;                // row_blocks * q_heads items, a CTA of the grid each
+    int32_t ranked;                    // row blocks go by length, else from the last to the first
+    int32_t wide_store;                // out rows are 32-byte aligned
     uint32_t negate;                   // scale < 0: the MMA negates Q, `scale` is positive
     float scale, softcap;
 };
 
 struct Bars {
-    uint32_t q, kv_full, kv_empty, s, p, o, done, clean;
+    uint32_t q, q_empty, kv_full, kv_empty, clean, s, p, o, item_full, item_empty, done, next;
     __device__ explicit Bars(uint32_t base)
-        : q(base), kv_full(base + 8), kv_empty(kv_full + 8 * STAGES), s(kv_empty + 8 * STAGES),
-          p(s + 16), o(p + 32), done(o + 16), clean(done + 8) {}
+        : q(base), q_empty(q + 16), kv_full(q_empty + 16), kv_empty(kv_full + 8 * STAGES),
+          clean(kv_empty + 8 * STAGES), s(clean + 8 * STAGES), p(s + 16), o(p + 32),
+          item_full(o + 16), item_empty(item_full + 8 * SLOTS), done(item_empty + 8 * SLOTS),
+          next(done + 8) {}
 };
+static_assert(16 + 16 + 24 * STAGES + 16 + 32 + 16 + 16 * SLOTS + 16 <= 8 * 40, "barrier area");
 
 // Rows [lo, hi) that row i sees; (0, 0) for a row behind the last document.
 // Safe for any content of cu_seqlens.
@@ -125,34 +142,54 @@ __device__ __forceinline__ int2 seen_rows(const Params& p, int i) {
     return make_int2(lo, hi);
 }
 
-// What every role needs to know of the CTA's work.  Key tile j is rows
-// kv0 + 128 j on; query tile t takes part in the key tiles [first[t], last[t]).
-struct Work {
-    int row0, head, kv0, tiles, first[2], last[2];
-    int clear0, clear1;                // key tiles that every valid row sees all of
+// What every role needs to know of an item.  Key tile j is rows kv0 + 128 j on;
+// query tile t takes part in the key tiles [first[t], last[t]).
+struct Item {
+    int row0, head, kv0, tiles;        // tiles < 0: there are no more items
+    int first[2], last[2];
+    int clear0, clear1;                // key tiles that every row of a document sees all of
+    int found;                         // run_clean() took something out
     // Whether some row does not see some key of tile j.
     __device__ bool edge(int j) const { return j < clear0 || j >= clear1; }
 };
+static_assert(sizeof(Item) <= 64, "item slot");
 
-// `seen[t]` holds the ranges of tile t's first and last row that belongs to a
-// document; `valid` rows of the CTA do.
-__device__ __forceinline__ Work make_work(const int2 (*seen)[2], int row0, int head, int valid) {
-    Work w;
+// Rows of documents, as a bound for the row numbers.
+__device__ __forceinline__ int document_rows(const Params& p) {
+    if (p.cu_seqlens == nullptr) return p.tokens;
+    return min(max(__ldg(p.cu_seqlens + p.docs), 0), p.tokens);
+}
+
+// One tile's key tiles from the ranges of its first and last row.
+__device__ __forceinline__ void tile_range(int2 head, int2 tail, int kv0, int& first, int& last) {
+    first = max(head.x - kv0, 0) / TILE;
+    last = max((tail.y - kv0 + TILE - 1) / TILE, first);
+}
+
+// The row block's item, by a whole warp; `valid` (> 0) of its rows belong to
+// documents.
+__device__ __forceinline__ Item make_item(const Params& p, int row0, int head, int valid) {
+    const int lane = threadIdx.x & 31;
+    int2 seen = make_int2(0, 0);
+    if (lane < 4) {
+        const int t = lane >> 1, end = min(valid, (t + 1) * TILE) - 1;
+        if (valid > t * TILE) seen = seen_rows(p, row0 + (lane & 1 ? end : t * TILE));
+    }
+    int2 at[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        at[k] = make_int2(__shfl_sync(0xffffffffu, seen.x, k), __shfl_sync(0xffffffffu, seen.y, k));
+    Item w;
     w.row0 = row0;
     w.head = head;
-    w.kv0 = seen[0][0].x;
-    w.clear0 = (max(seen[valid > TILE][1].x - w.kv0, 0) + TILE - 1) / TILE;
-    w.clear1 = max(seen[0][0].y - w.kv0, 0) / TILE;
-    w.tiles = 0;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        w.first[t] = w.last[t] = 0;
-        if (valid > t * TILE) {
-            w.first[t] = max(seen[t][0].x - w.kv0, 0) / TILE;
-            w.last[t] = max((seen[t][1].y - w.kv0 + TILE - 1) / TILE, w.first[t]);
-        }
-        w.tiles = max(w.tiles, w.last[t]);
-    }
+    w.kv0 = at[0].x;
+    w.clear0 = (max((valid > TILE ? at[3].x : at[1].x) - w.kv0, 0) + TILE - 1) / TILE;
+    w.clear1 = max(at[0].y - w.kv0, 0) / TILE;
+    w.first[1] = w.last[1] = 0;
+    tile_range(at[0], at[1], w.kv0, w.first[0], w.last[0]);
+    if (valid > TILE) tile_range(at[2], at[3], w.kv0, w.first[1], w.last[1]);
+    w.tiles = max(w.last[0], w.last[1]);
+    w.found = 0;
     return w;
 }
 
@@ -317,42 +354,144 @@ __device__ __forceinline__ f32x2 ex2_poly(f32x2 x) {
                         __int_as_float((__float_as_int(n.y) << 23) + 0x3f800000)));
 }
 
+// One sector with one instruction: 32-byte aligned.
+__device__ __forceinline__ void store_32_bytes(void* p, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                   "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 __device__ __forceinline__ uint32_t pack_bf16x2_rn(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// ------------------------------------------------------------ loads
-// Ring order: K_0, V_0, K_1, V_1, ...
-__device__ void run_loads(const Params& p, const Work& w, uint8_t* smem, const Bars& b,
-                          volatile int* abort_flag) {
+// ------------------------------------------------------------ items and loads
+// Takes over a CTA of this grid that has not started yet; 16 bytes of answer,
+// counted on `bar`.
+__device__ __forceinline__ void claim_cta(uint32_t answer, uint32_t bar) {
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128"
+        " [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+
+// The x index of the CTA taken over, -1 if there was none left.
+__device__ __forceinline__ int claimed_cta(uint32_t answer) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b64 lo, hi;\n\t"
+        "ld.shared.v2.b64 {lo, hi}, [%2];\n\tmov.b128 r, {lo, hi};\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %1, 1, 0, p;\n\tmov.u32 %0, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, r;\n\t}"
+        : "=r"(x), "=r"(got) : "r"(answer) : "memory");
+    return got ? static_cast<int>(x) : -1;
+}
+
+// Ring order per item: K_0, V_0, K_1, V_1, ...  The whole warp works out the
+// items, its first lane loads.
+__device__ void run_loads(const Params& p, uint8_t* smem, const Bars& b, volatile int* abort_flag) {
     const uint32_t q = smem_u32(smem + OFF_Q), ring = smem_u32(smem + OFF_KV);
-    const int q_col = w.head * D, kv_col = w.head / p.group * D;
-    mbar_arrive_expect_tx(b.q, 2 * TILE_BYTES);
-    for (int t = 0; t < 2; ++t)
-        for (int c = 0; c < 2; ++c)
-            tma_load_2d(q + t * TILE_BYTES + c * BOX_BYTES, &p.tm_q, b.q, q_col + 64 * c,
-                        w.row0 + t * TILE);
-    int i = 0;
-    for (; i < 2 * w.tiles; ++i) {
-        const int s = i % STAGES, use = i / STAGES;
-        if (!fu_wait_parity(b.kv_empty + 8 * s, (use & 1) ^ 1, abort_flag, p.timeout_ns, p.status,
-                            W_KV_EMPTY))
-            break;
-        mbar_arrive_expect_tx(b.kv_full + 8 * s, TILE_BYTES);
-        for (int c = 0; c < 2; ++c)
-            tma_load_2d(ring + s * TILE_BYTES + c * BOX_BYTES, i & 1 ? &p.tm_v : &p.tm_k,
-                        b.kv_full + 8 * s, kv_col + 64 * c, w.kv0 + (i >> 1) * TILE);
+    const uint8_t* rank = smem + OFF_RANK;
+    const int lane = threadIdx.x & 31;
+    const int rows = document_rows(p);
+    const auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool {
+        return __all_sync(0xffffffffu, fu_wait_parity(bar, parity, abort_flag, p.timeout_ns,
+                                                      p.status, where));
+    };
+    int n = 0, stage = 0;              // items handed out, ring stage
+    uint32_t use = 0;                  // the stage's phase
+    int loads = 0;                     // ring loads issued, up to STAGES
+    int q_loads[2] = {0, 0};
+    bool ok = true;
+    int k = blockIdx.x;                // the item; < 0: there are no more
+    uint32_t asked = 0;                // phase of `next`
+    // The next item is that of a CTA that has not started, which then never does; asked
+    // for when this one's last loads are out.
+    const uint32_t answer = smem_u32(smem + OFF_MISC + 16);
+    const auto claim = [&]() {
+        if (lane == 0) {
+            mbar_arrive_expect_tx(b.next, 16);
+            claim_cta(answer, b.next);
+        }
+        if (!(ok = wait(b.next, asked, W_ITEM))) return -1;
+        asked ^= 1;
+        const int next = claimed_cta(answer);
+        fence_proxy_async_smem();
+        __syncwarp();
+        return next;
+    };
+    while (ok) {
+        Item w;
+        w.tiles = -1;
+        if (k >= 0) {
+            const int block = k / p.q_heads;
+            const int head = k - block * p.q_heads;
+            const int row0 = (p.ranked ? rank[block] : p.row_blocks - 1 - block) * ROWS;
+            const int valid = min(rows - row0, ROWS);
+            if (valid > 0) w = make_item(p, row0, head, valid);
+            if (w.tiles <= 0) {        // (0: cu_seqlens that make no sense)
+                k = claim();
+                continue;
+            }
+        }
+        const int slot = n % SLOTS;
+        const uint32_t phase = (n / SLOTS) & 1;
+        if (!(ok = wait(b.item_empty + 8 * slot, phase ^ 1, W_SLOT))) break;
+        if (lane == 0) {
+            *reinterpret_cast<Item*>(smem + OFF_ITEM + 64 * slot) = w;
+            mbar_arrive(b.item_full + 8 * slot);
+        }
+        __syncwarp();
+        if (k < 0) break;
+        const int q_col = w.head * D, kv_col = w.head / p.group * D;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            if (!ok || !(ok = wait(b.q_empty + 8 * t, (n & 1) ^ 1, W_Q_EMPTY))) break;
+            ++q_loads[t];
+            if (lane == 0) {
+                mbar_arrive_expect_tx(b.q + 8 * t, TILE_BYTES);
+                for (int c = 0; c < 2; ++c)
+                    tma_load_2d(q + t * TILE_BYTES + c * BOX_BYTES, &p.tm_q, b.q + 8 * t,
+                                q_col + 64 * c, w.row0 + t * TILE);
+            }
+            if (t == 1) ++n;
+            // The first keys go between the two tiles' rows.
+            for (int i = t; ok && i < (t == 0 ? 1 : 2 * w.tiles); ++i) {
+                if (!(ok = wait(b.kv_empty + 8 * stage, use ^ 1, W_KV_EMPTY))) break;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(b.kv_full + 8 * stage, TILE_BYTES);
+                    for (int c = 0; c < 2; ++c)
+                        tma_load_2d(ring + stage * TILE_BYTES + c * BOX_BYTES,
+                                    i & 1 ? &p.tm_v : &p.tm_k, b.kv_full + 8 * stage,
+                                    kv_col + 64 * c, w.kv0 + (i >> 1) * TILE);
+                }
+                loads = min(loads + 1, STAGES);
+                if (++stage == STAGES) {
+                    stage = 0;
+                    use ^= 1;
+                }
+            }
+        }
+        if (ok) k = claim();
     }
     // What was issued must land before shared memory is released, whatever the
     // other roles did.
-    drain_wait(b.q, 0, p.timeout_ns, p.status);
-    for (int k = i > STAGES ? i - STAGES : 0; k < i; ++k)
-        drain_wait(b.kv_full + 8 * (k % STAGES), (k / STAGES) & 1, p.timeout_ns, p.status);
+    for (int k = 0; k < loads; ++k) {
+        if (--stage < 0) {
+            stage = STAGES - 1;
+            use ^= 1;
+        }
+        drain_wait(b.kv_full + 8 * stage, use, p.timeout_ns, p.status);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+        if (q_loads[t] > 0) drain_wait(b.q + 8 * t, (q_loads[t] - 1) & 1, p.timeout_ns, p.status);
 }
 
 // ------------------------------------------------------------ MMA
-__device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t tmem, const Bars& b,
+__device__ void run_mma(const Params& p, uint8_t* smem, uint32_t tmem, const Bars& b,
                         volatile int* abort_flag) {
     // S = Q K^T: both K-major.  O += P V: P from TMEM, V [keys, dims] MN-major.
     const uint32_t idesc_s = make_idesc_bf16_f32(TILE, TILE, false, false) | (p.negate << 13);
@@ -365,39 +504,60 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
                                                       p.status, where));
     };
     const auto same = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
-    const int first0 = same(w.first[0]), first1 = same(w.first[1]);
-    const int last0 = same(w.last[0]), last1 = same(w.last[1]);
-    const int tiles = same(w.tiles), clear0 = same(w.clear0), clear1 = same(w.clear1);
     tmem = same(tmem);
     uint32_t p_phase0 = 0, p_phase1 = 0;
-    // Ring stages and phases of V_j and K_(j+1), and the count of V_j.
-    int sv = STAGES - 1, sk = 0, sc = STAGES - 1;
-    uint32_t v_phase = 1, k_phase = 0, c_phase = 1;
-    const auto v_arrived = [&](int j) {
-        if (j < 0 || j >= tiles) return true;
-        const bool edge = j < clear0 || j >= clear1;
-        return wait(edge ? b.clean + 8 * sc : b.kv_full + 8 * sv, edge ? c_phase : v_phase,
-                    edge ? W_CLEAN : W_KV_FULL);
+    // Ring stages and phases of the next V and the next K, and the next V's count.
+    int sk = 0, sv = 1, sc = 0;
+    uint32_t k_phase = 0, v_phase = 0, c_phase = 0;
+    // An item's fields; `tiles` < 0 when there are no more.
+    struct Range { int first0, first1, last0, last1, tiles, clear0, clear1; };
+    int n = 0;                         // items taken
+    bool ok = true;
+    const auto take = [&]() {
+        Range r = {0, 0, 0, 0, -1, 0, 0};
+        const int slot = n % SLOTS;
+        if (!(ok = wait(b.item_full + 8 * slot, (n / SLOTS) & 1, W_ITEM))) return r;
+        const Item& w = *reinterpret_cast<const Item*>(smem + OFF_ITEM + 64 * slot);
+        r.first0 = same(w.first[0]);
+        r.first1 = same(w.first[1]);
+        r.last0 = same(w.last[0]);
+        r.last1 = same(w.last[1]);
+        r.tiles = same(w.tiles);
+        r.clear0 = same(w.clear0);
+        r.clear1 = same(w.clear1);
+        __syncwarp();
+        if (one) mbar_arrive(b.item_empty + 8 * slot);
+        ++n;
+        return r;
     };
-    bool ok = wait(b.q, 0, W_Q);
-    // Step j: the products P V of key tile j, each followed by the same query
-    // tile's scores of key tile j + 1.
+    // A step takes, for one query tile and then the other, the product P V of key
+    // tile j and the scores of the key tile after it: j + 1, or the first of the next
+    // item, whose work on the first query tile so begins while the second still has
+    // the last key tiles of this one to do.
+    Range w = {0, 0, 0, 0, 0, 0, 0}, next = take();
+    int j = -1;
 #pragma unroll 1
-    for (int j = -1; ok && j < tiles; ++j) {
+    while (ok) {
+        const bool turn = j + 1 == w.tiles;            // scores for the next item
+        if (turn && j >= 0) next = take();
+        if (!ok || (turn && j < 0 && next.tiles < 0)) break;
+        const int jn = turn ? 0 : j + 1;
+        const bool more = turn ? next.tiles > 0 : true;
         const uint32_t v_lo = desc_lo(ring + sv * TILE_BYTES, BOX_BYTES);   // 64-column boxes
         const uint32_t k_lo = desc_lo(ring + sk * TILE_BYTES, 16);
         const uint32_t v_empty = b.kv_empty + 8 * sv, k_empty = b.kv_empty + 8 * sk;
+        if (j >= 0) {
+            const bool edge = j < w.clear0 || j >= w.clear1;
+            ok = wait(edge ? b.clean + 8 * sc : b.kv_full + 8 * sv, edge ? c_phase : v_phase,
+                      edge ? W_CLEAN : W_KV_FULL);
+            if (!ok) break;
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int first = t ? first1 : first0, last = t ? last1 : last0;
+            const int first = t ? w.first1 : w.first0, last = t ? w.last1 : w.last0;
+            const int firstn = turn ? (t ? next.first1 : next.first0) : first;
+            const int lastn = turn ? (t ? next.last1 : next.last0) : last;
             uint32_t& p_phase = t ? p_phase1 : p_phase0;
-            if (t == 1) {
-                // The next step's V is looked for while the first query tile's
-                // products run; K, which comes later, just before it is needed.
-                sv = sv + 2 < STAGES ? sv + 2 : (v_phase ^= 1, sv + 2 - STAGES);
-                sc = sc + 1 < STAGES ? sc + 1 : (c_phase ^= 1, 0);
-                if (!(ok = v_arrived(j + 1))) break;
-            }
             if (j >= first && j < last) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -414,9 +574,10 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
                 if (j + 1 == last) commit(one, b.o + 8 * t);
             }
             if (t == 1 && j >= 0) commit(one, v_empty);
-            if (t == 0 && j + 1 < tiles && !(ok = wait(b.kv_full + 8 * sk, k_phase, W_KV_FULL)))
-                break;
-            if (j + 1 >= first && j + 1 < last) {
+            if (!more) continue;
+            if (turn && !(ok = wait(b.q + 8 * t, (n - 1) & 1, W_Q))) break;
+            if (t == 0 && !(ok = wait(b.kv_full + 8 * sk, k_phase, W_KV_FULL))) break;
+            if (jn >= firstn && jn < lastn) {
                 tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
@@ -426,9 +587,18 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
                 }
                 commit(one, b.s + 8 * t);
             }
-            if (t == 1 && j + 1 < tiles) commit(one, k_empty);
+            // The tile's rows are no longer needed (a tile without rows: at once).
+            if (lastn > firstn ? jn + 1 == lastn : turn) commit(one, b.q_empty + 8 * t);
+            if (t == 1) commit(one, k_empty);
+        }
+        if (!ok || !more) break;
+        if (j >= 0) {
+            sv = sv + 2 < STAGES ? sv + 2 : (v_phase ^= 1, sv + 2 - STAGES);
+            sc = sc + 1 < STAGES ? sc + 1 : (c_phase ^= 1, 0);
         }
         sk = sk + 2 < STAGES ? sk + 2 : (k_phase ^= 1, sk + 2 - STAGES);
+        if (turn) w = next;
+        j = jn;
     }
     // Every MMA this warp issued must finish before TMEM is released.
     commit(one, b.done);
@@ -438,71 +608,98 @@ __device__ void run_mma(const Params& p, const Work& w, uint8_t* smem, uint32_t 
 // ------------------------------------------------------------ V at a mask's edge
 // Every V tile is counted (on a ring of barriers of its own), so that neither
 // side gets more than the ring ahead; only those at an edge are looked at.
-__device__ void run_clean(const Params& p, const Work& w, uint8_t* smem, const Bars& b,
-                          volatile int* abort_flag, volatile int* found) {
+__device__ void run_clean(const Params& p, uint8_t* smem, const Bars& b,
+                          volatile int* abort_flag) {
     const int me = threadIdx.x & 63;
-    for (int j = 0; j < w.tiles; ++j) {
-        const int i = 2 * j + 1, s = i % STAGES;
-        if (!fu_wait_parity(b.kv_full + 8 * s, (i / STAGES) & 1, abort_flag, p.timeout_ns, p.status,
-                            W_KV_FULL))
-            return;
-        uint4* v = reinterpret_cast<uint4*>(smem + OFF_KV + s * TILE_BYTES);
-        bool wrote = false;
+    int stage = 1, count = 0;          // of the next V tile: ring stage, place on its own ring
+    uint32_t use = 0;
+    for (int n = 0;; ++n) {
+        const int slot = n % SLOTS;
+        bool ok = fu_wait_parity(b.item_full + 8 * slot, (n / SLOTS) & 1, abort_flag, p.timeout_ns,
+                                 p.status, W_ITEM);
+        if (!__all_sync(0xffffffffu, ok)) return;
+        Item& w = *reinterpret_cast<Item*>(smem + OFF_ITEM + 64 * slot);
+        const int tiles = w.tiles;
+        for (int j = 0; j < tiles; ++j) {
+            ok = fu_wait_parity(b.kv_full + 8 * stage, use, abort_flag, p.timeout_ns, p.status,
+                                W_KV_FULL);
+            if (!__all_sync(0xffffffffu, ok)) return;
+            if (w.edge(j)) {
+                uint4* v = reinterpret_cast<uint4*>(smem + OFF_KV + stage * TILE_BYTES);
+                // A BF16 is not finite if its exponent bits are all set; one more then
+                // carries into the sign's place.
+                uint32_t bad = 0;
 #pragma unroll 8
-        for (int o = me; o < (w.edge(j) ? TILE_BYTES / 16 : 0); o += 64) {
-            uint4 x = v[o];
-            uint32_t* word = &x.x;
-            bool odd = false;
+                for (int o = me; o < TILE_BYTES / 16; o += 64) {
+                    const uint4 x = v[o];
+                    bad |= ((x.x & 0x7f807f80u) + 0x00800080u) | ((x.y & 0x7f807f80u) + 0x00800080u) |
+                           ((x.z & 0x7f807f80u) + 0x00800080u) | ((x.w & 0x7f807f80u) + 0x00800080u);
+                }
+                if (bad & 0x80008000u) {
+#pragma unroll 1
+                    for (int o = me; o < TILE_BYTES / 16; o += 64) {
+                        uint4 x = v[o];
+                        uint32_t* word = &x.x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                // A BF16 is not finite if its exponent bits are all set.
-                const uint32_t bad = __vcmpeq2(word[k] & 0x7f807f80u, 0x7f807f80u);
-                word[k] &= ~bad;
-                odd = odd || bad != 0;
+                        for (int k = 0; k < 4; ++k)
+                            word[k] &= ~__vcmpeq2(word[k] & 0x7f807f80u, 0x7f807f80u);
+                        v[o] = x;
+                    }
+                    *const_cast<volatile int*>(&w.found) = 1;
+                    fence_proxy_async_smem();
+                }
             }
-            if (odd) {
-                v[o] = x;
-                wrote = true;
+            __syncwarp();
+            if ((me & 31) == 0) mbar_arrive(b.clean + 8 * count);
+            if (++count == STAGES) count = 0;
+            stage += 2;
+            if (stage >= STAGES) {
+                stage -= STAGES;
+                use ^= 1;
             }
-        }
-        if (wrote) {
-            *found = 1;
-            fence_proxy_async_smem();
         }
         __syncwarp();
-        if ((me & 31) == 0) mbar_arrive(b.clean + 8 * (j % STAGES));
+        if ((me & 31) == 0) mbar_arrive(b.item_empty + 8 * slot);
+        if (tiles < 0) return;
     }
 }
 
 // ------------------------------------------------------------ softmax
 // kMode: 1 scores capped by a tanh, 2 lowered with distance (3 both).
 template <int kMode>
-__device__ void run_softmax(const Params& p, const Work& w, uint8_t* smem, uint32_t tmem,
-                            const Bars& b, int t, int2 seen, bool valid,
-                            volatile int* abort_flag, volatile int* found) {
-    const int first = t ? w.first[1] : w.first[0], last = t ? w.last[1] : w.last[0];
+__device__ void run_softmax(const Params& p, uint8_t* smem, uint32_t tmem, const Bars& b, int t,
+                            volatile int* abort_flag) {
     const int lane = threadIdx.x & 31;
     const int warp = (threadIdx.x >> 5) & 3;              // of this tile
-    const int row = w.row0 + t * TILE + warp * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t tm_s = tmem + TM_S + t * TILE + lanes, tm_o = tmem + TM_O + t * TILE + lanes;
     // Scores in units of log2: x = c * s here, m in the units of s (so c m is
     // its logarithm), or with a cap or a bias x = s, c = 1.
     const float c = kMode ? 1.f : fmaxf(p.scale * LOG2E, 1e-30f);
-    const float slope =
-        kMode & 2 ? __ldg(p.alibi_slopes + w.head) * LOG2E : 0.f;
     const float lin = p.scale * LOG2E;
     const float to_cap = kMode & 1 ? p.scale / p.softcap : 0.f;
+    const auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool {
+        return __all_sync(0xffffffffu, fu_wait_parity(bar, parity, abort_flag, p.timeout_ns,
+                                                      p.status, where));
+    };
+    uint32_t phase = 0, o_phase = 0;
+    for (int n = 0;; ++n) {
+    const int slot = n % SLOTS;
+    if (!wait(b.item_full + 8 * slot, (n / SLOTS) & 1, W_ITEM)) return;
+    const Item& w = *reinterpret_cast<const Item*>(smem + OFF_ITEM + 64 * slot);
+    if (w.tiles < 0) return;
+    const int first = w.first[t], last = w.last[t], kv0 = w.kv0;
+    const int row = w.row0 + t * TILE + warp * 32 + lane;
+    const float slope = kMode & 2 ? __ldg(p.alibi_slopes + w.head) * LOG2E : 0.f;
+    const int2 seen = row < p.tokens ? seen_rows(p, row) : make_int2(0, 0);
+    const bool valid = seen.x < seen.y;
     // A row without a document is computed like one that sees everything, and
     // not stored.
     const int lo = valid ? seen.x : INT_MIN / 2, hi = valid ? seen.y : INT_MAX / 2;
 
     float m = -INFINITY, l = 0.f;
-    uint32_t phase = 0;
-    bool ok = true;
     for (int j = first; j < last; ++j) {
-        ok = fu_wait_parity(b.s + 8 * t, phase, abort_flag, p.timeout_ns, p.status, W_S);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if (!wait(b.s + 8 * t, phase, W_S)) return;
         phase ^= 1;
         tc_fence_after();
         uint32_t r[TILE];
@@ -511,7 +708,7 @@ __device__ void run_softmax(const Params& p, const Work& w, uint8_t* smem, uint3
         for (int k = 0; k < 4; ++k)
             tmem_ld_32cols(tm_s + 32 * k, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * k));
         tmem_ld_wait();
-        const int k0 = w.kv0 + j * TILE;
+        const int k0 = kv0 + j * TILE;
         if (kMode & 1) {
             // cap tanh(z), z = scale s / cap.  Where all of the warp's |z| are at
             // most 1 (scores below the cap, the ordinary case) by an odd polynomial
@@ -629,59 +826,57 @@ __device__ void run_softmax(const Params& p, const Work& w, uint8_t* smem, uint3
         const float2 total = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
         l += total.x + total.y;
     }
-    if (first == last || !ok) return;
-
-    // out = O / l, through this tile's Q rows in shared memory (no longer
-    // needed): a thread writes its row, then the warp's 32 rows leave as whole
-    // 256-byte rows.
-    ok = fu_wait_parity(b.o + 8 * t, 0, abort_flag, p.timeout_ns, p.status, W_O);
-    if (!__all_sync(0xffffffffu, ok)) return;
-    tc_fence_after();
-    const float inv = 1.f / l;
-    const bool poison = *found != 0;
-    uint8_t* stage = smem + OFF_Q + t * TILE_BYTES + warp * 32 * 256;
+    if (first < last) {
+        // out = O / l, a row of 256 bytes a thread.
+        if (!wait(b.o + 8 * t, o_phase, W_O)) return;
+        o_phase ^= 1;
+        tc_fence_after();
+        const float inv = 1.f / l;
+        const bool poison = *const_cast<const volatile int*>(&w.found) != 0;
+        __nv_bfloat16* dst = p.out + static_cast<int64_t>(row) * p.out_stride + w.head * D;
 #pragma unroll 1
-    for (int k = 0; k < 4; ++k) {
-        uint32_t o[32];
-        tmem_ld_32cols(tm_o + 32 * k, o);
-        tmem_ld_wait();
+        for (int k = 0; k < 4; ++k) {
+            uint32_t o[32];
+            tmem_ld_32cols(tm_o + 32 * k, o);
+            tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * inv);
-        if (poison && valid) {
-            // What run_clean() took out, for the rows that see it.
-            for (int j = first; j < last; ++j) {
-                if (!w.edge(j)) continue;
-                const int a = max(lo, w.kv0 + j * TILE), e = min(hi, w.kv0 + (j + 1) * TILE);
-                for (int key = a; key < e; ++key) {
-                    const __nv_bfloat16* v = p.v + key * p.v_stride + w.head / p.group * D + 32 * k;
+            for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * inv);
+            if (poison && valid) {
+                // What run_clean() took out, for the rows that see it.
+                for (int j = first; j < last; ++j) {
+                    if (!w.edge(j)) continue;
+                    const int a = max(lo, kv0 + j * TILE), e = min(hi, kv0 + (j + 1) * TILE);
+                    for (int key = a; key < e; ++key) {
+                        const __nv_bfloat16* v =
+                            p.v + key * p.v_stride + w.head / p.group * D + 32 * k;
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) {
-                        const float x = __bfloat162float(v[q]);
-                        if (!isfinite(x)) o[q] = __float_as_uint(__uint_as_float(o[q]) + x);
+                        for (int q = 0; q < 32; ++q) {
+                            const float x = __bfloat162float(v[q]);
+                            if (!isfinite(x)) o[q] = __float_as_uint(__uint_as_float(o[q]) + x);
+                        }
                     }
                 }
             }
-        }
+            uint32_t packed[16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int chunk = 4 * k + q;
-            const uint32_t* x = o + 8 * q;
-            *reinterpret_cast<uint4*>(stage + lane * 256 + ((chunk ^ (lane & 7)) << 4)) = make_uint4(
-                pack_bf16x2_rn(__uint_as_float(x[0]), __uint_as_float(x[1])),
-                pack_bf16x2_rn(__uint_as_float(x[2]), __uint_as_float(x[3])),
-                pack_bf16x2_rn(__uint_as_float(x[4]), __uint_as_float(x[5])),
-                pack_bf16x2_rn(__uint_as_float(x[6]), __uint_as_float(x[7])));
+            for (int q = 0; q < 16; ++q)
+                packed[q] = pack_bf16x2_rn(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1]));
+            if (!valid) continue;
+            if (p.wide_store) {
+                store_32_bytes(dst + 32 * k, packed);
+                store_32_bytes(dst + 32 * k + 16, packed + 8);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<uint4*>(dst + 32 * k + 8 * q) = make_uint4(
+                        packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+            }
         }
+        // The next product into O comes behind weights of these warps.
+        tc_fence_before();
     }
-    const uint32_t stored = __ballot_sync(0xffffffffu, valid);
     __syncwarp();
-    __nv_bfloat16* dst = p.out + static_cast<int64_t>(row - lane) * p.out_stride + w.head * D;
-#pragma unroll 4
-    for (int r = lane >> 4; r < 32; r += 2) {
-        const int chunk = lane & 15;
-        if (stored >> r & 1)
-            *reinterpret_cast<uint4*>(dst + r * p.out_stride + 8 * chunk) =
-                *reinterpret_cast<const uint4*>(stage + r * 256 + ((chunk ^ (r & 7)) << 4));
+    if (lane == 0) mbar_arrive(b.item_empty + 8 * slot);
     }
 }
 
@@ -694,29 +889,32 @@ attention_kernel(const __grid_constant__ Params p) {
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int warp = threadIdx.x >> 5;
     const Bars b(smem_u32(smem + OFF_BAR));
-    int2 (*seen)[2] = reinterpret_cast<int2 (*)[2]>(smem + OFF_SEEN);
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + OFF_MISC);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + OFF_MISC + 4);
-    volatile int* found = reinterpret_cast<volatile int*>(smem + OFF_MISC + 8);
 
     // Prologue: shared memory, TMEM and parameters only (it may overlap the
     // previous kernel of the stream under a programmatic dependent launch).
     if (threadIdx.x == 0) {
-        mbar_init(b.q, 1);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(b.kv_full + 8 * s, 1);
             mbar_init(b.kv_empty + 8 * s, 1);
             mbar_init(b.clean + 8 * s, 2);
         }
         for (int t = 0; t < 2; ++t) {
+            mbar_init(b.q + 8 * t, 1);
+            mbar_init(b.q_empty + 8 * t, 1);
             mbar_init(b.s + 8 * t, 1);
             mbar_init(b.p + 16 * t, 4);
             mbar_init(b.p + 16 * t + 8, 4);
             mbar_init(b.o + 8 * t, 1);
         }
+        for (int k = 0; k < SLOTS; ++k) {
+            mbar_init(b.item_full + 8 * k, 1);
+            mbar_init(b.item_empty + 8 * k, 11);       // warps: 8 softmax, MMA, 2 cleaning
+        }
         mbar_init(b.done, 1);
+        mbar_init(b.next, 1);
         *abort_flag = 0;
-        *found = 0;
         fence_mbar_init();
         tma_prefetch_desc(&p.tm_q);
         tma_prefetch_desc(&p.tm_k);
@@ -730,10 +928,6 @@ attention_kernel(const __grid_constant__ Params p) {
     grid_dependency_wait();
     grid_launch_dependents();
 
-    // The longest rows first: with a causal mask the last CTAs to start then
-    // have the least to do.
-    const int head = blockIdx.x % p.q_heads;
-    const int row0 = (gridDim.x / p.q_heads - 1 - blockIdx.x / p.q_heads) * ROWS;
     if (blockIdx.x == 0 && p.cu_seqlens != nullptr) {
         for (int d = threadIdx.x; d <= p.docs; d += NUM_THREADS) {
             const int x = __ldg(p.cu_seqlens + d);
@@ -742,38 +936,53 @@ attention_kernel(const __grid_constant__ Params p) {
                 report_status(p.status, FU_DEV_LENGTHS, W_CU_SEQLENS);
         }
     }
-    int rows = p.tokens;                               // rows of documents
-    if (p.cu_seqlens != nullptr) rows = min(max(__ldg(p.cu_seqlens + p.docs), 0), p.tokens);
-    const int valid = min(rows - row0, ROWS);
-    int2 mine = make_int2(0, 0);
-    if (warp < 8) {
-        const int i = threadIdx.x, t = i / TILE;
-        if (row0 + i < p.tokens) mine = seen_rows(p, row0 + i);
-        if (i == t * TILE) seen[t][0] = mine;
-        if (i == min(valid, (t + 1) * TILE) - 1) seen[t][1] = mine;
+    if (p.ranked) {
+        // Row blocks by the key tiles that their two query tiles walk, longest
+        // first: each counts those that go before it.
+        int* cost = reinterpret_cast<int*>(smem + OFF_KV);
+        const int me = threadIdx.x, rows = document_rows(p);
+        int mine = 0;
+        if (me < p.row_blocks) {
+            const int valid = min(rows - me * ROWS, ROWS);
+            int kv0 = 0;
+            for (int t = 0; t < 2 && valid > t * TILE; ++t) {
+                const int2 head = seen_rows(p, me * ROWS + t * TILE);
+                const int2 tail = seen_rows(p, me * ROWS + min(valid, (t + 1) * TILE) - 1);
+                if (t == 0) kv0 = head.x;
+                int first, last;
+                tile_range(head, tail, kv0, first, last);
+                mine += last - first;
+            }
+            cost[me] = mine;
+        }
+        __syncthreads();
+        if (me < p.row_blocks) {
+            int before = 0;
+            for (int k = 0; k < p.row_blocks; ++k) {
+                const int other = cost[k];
+                before += other > mine || (other == mine && k > me);
+            }
+            smem[OFF_RANK + before] = static_cast<uint8_t>(me);
+        }
+        fence_proxy_async_smem();                      // the ring's loads go over `cost`
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
 
-    if (valid > 0) {
-        const Work w = make_work(seen, row0, head, valid);
-        if (warp < 8) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
-            run_softmax<kMode>(p, w, smem, tmem, b, warp >> 2, mine, mine.x < mine.y, abort_flag,
-                               found);
-        } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-            if (warp == 8) {
-                if ((threadIdx.x & 31) == 0) run_loads(p, w, smem, b, abort_flag);
-            } else if (warp == 9) {
-                run_mma(p, w, smem, tmem, b, abort_flag);
-            } else {
-                run_clean(p, w, smem, b, abort_flag, found);
-            }
-            __syncwarp();
-        }
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
+        run_softmax<kMode>(p, smem, tmem, b, warp >> 2, abort_flag);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+        if (warp == 8)
+            run_loads(p, smem, b, abort_flag);
+        else if (warp == 9)
+            run_mma(p, smem, tmem, b, abort_flag);
+        else
+            run_clean(p, smem, b, abort_flag);
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -802,18 +1011,18 @@ static int encode_rows(CUtensorMap* map, const void* base, int64_t rows, int64_t
 
 typedef void (*Kernel)(const Params);
 
-// Raises the kernels' shared-memory limit once per device.
+// Raises the kernels' shared-memory limit once per device (the current one).
 static cudaError_t prepare(int device) {
-    static std::atomic<uint64_t> done{0};
-    const uint64_t bit = 1ull << (device & 63);
-    if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    constexpr int MAX_DEVICES = 64;
+    static std::atomic<bool> done[MAX_DEVICES];
+    if (device < MAX_DEVICES && done[device].load(std::memory_order_acquire)) return cudaSuccess;
     for (Kernel k : {attention_kernel<0>, attention_kernel<1>, attention_kernel<2>,
                      attention_kernel<3>}) {
         cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              SMEM_ALLOC);
         if (e != cudaSuccess) return e;
     }
-    if (device < 64) done.fetch_or(bit, std::memory_order_release);
+    if (device < MAX_DEVICES) done[device].store(true, std::memory_order_release);
     return cudaSuccess;
 }
 
@@ -880,6 +1089,9 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
     p.q_heads = a->q_heads;
     p.group = a->q_heads / a->kv_heads;
     p.causal = a->causal;
+    p.row_blocks = static_cast<int32_t>((a->tokens + attention::ROWS - 1) / attention::ROWS);
+    p.ranked = a->cu_seqlens != nullptr && p.row_blocks > 1 && p.row_blocks <= attention::MAX_RANKED;
+    p.wide_store = (reinterpret_cast<uintptr_t>(a->out) | a->out_stride * 2) % 32 == 0;
     p.negate = a->scale < 0.f ? 1u : 0u;
     p.scale = std::fabs(a->scale);
     p.softcap = a->softcap;
