@@ -73,9 +73,9 @@ constexpr int SMEM_ALLOC = SMEM_BYTES + 1024;   // room to align the base to 1 K
 static_assert(SMEM_ALLOC <= 232448, "exceeds the 227 KiB per-CTA shared memory limit");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TM_S = 0, TM_O = 256;        // + 128 * tile
-// Registers: 3 warpgroups launch with 168 each; the softmax takes 216, the
-// others keep 72 (216 + 216 + 72 = 3 * 168).
-constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
+// Registers: 3 warpgroups launch with 168 each; the softmax takes 208, the
+// others keep 88 (208 + 208 + 88 = 3 * 168); neither spills.
+constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 88;
 constexpr float LOG2E = 1.4426950408889634f;
 // Every so manieth pair of a row's weights is computed on the FMA pipes
 // (ex2_poly), the others by the special-function unit, whose 16 results per
@@ -678,6 +678,13 @@ __device__ void run_softmax(const Params& p, uint8_t* smem, uint32_t tmem, const
     const float c = kMode ? 1.f : fmaxf(p.scale * LOG2E, 1e-30f);
     const float lin = p.scale * LOG2E;
     const float to_cap = kMode & 1 ? p.scale / p.softcap : 0.f;
+    const float z2 = to_cap * to_cap;
+    // tanh(z) = z + .. to z^7 for |z| <= 1/2, off by 2e-7, as a polynomial in s (the last
+    // coefficient would underflow for a cap above some 10^4 times the scale's inverse).
+    const float cap_low[4] = {lin, -0.33326461911201477f * lin * z2,
+                              0.13185861706733704f * lin * z2 * z2,
+                              -0.04422929883003235f * lin * z2 * z2 * z2};
+    const bool cap_small = to_cap >= 1e-5f;
     const auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool {
         return __all_sync(0xffffffffu, fu_wait_parity(bar, parity, abort_flag, p.timeout_ns,
                                                       p.status, where));
@@ -710,21 +717,28 @@ __device__ void run_softmax(const Params& p, uint8_t* smem, uint32_t tmem, const
         tmem_ld_wait();
         const int k0 = kv0 + j * TILE;
         if (kMode & 1) {
-            // cap tanh(z), z = scale s / cap.  Where all of the warp's |z| are at
-            // most 1 (scores below the cap, the ordinary case) by an odd polynomial
-            // of degree 11, off by 7e-7; else as cap (1 - 2 / (1 + 2^(2 log2(e) z))),
-            // off by 2^-22: absolute errors in both, which is what a score needs.
-            // The second takes three special-function results per score with the
-            // weight's, 4.5 us per tile against 1.1 us without a cap.
+            // cap tanh(z), z = scale s / cap.  Where all of the warp's |z| are at most
+            // 1/2 (scores well below the cap, the ordinary case) by an odd polynomial
+            // of degree 7, at most 1 by one of degree 11, off by 7e-7; else as
+            // cap (1 - 2 / (1 + 2^(2 log2(e) z))), off by 2^-22: absolute errors in all,
+            // which is what a score needs.  A packed FMA takes its pipe two clocks, so
+            // the polynomials' length is what a cap costs; the last form takes three
+            // special-function results per score with the weight's.
             float far = 0.f;
 #pragma unroll
             for (int k = 0; k < TILE; k += 2) far = max3(far, fabsf(s[k]), fabsf(s[k + 1]));
-            if (__any_sync(0xffffffffu, !(far * to_cap <= 1.f))) {
-                const float in = 2.f * LOG2E * to_cap, out = p.softcap * LOG2E;
+            if (__all_sync(0xffffffffu, cap_small && far * to_cap <= 0.5f)) {
 #pragma unroll
-                for (int k = 0; k < TILE; ++k)
-                    s[k] = fmaf(-2.f * out, __fdividef(1.f, 1.f + ex2(s[k] * in)), out);
-            } else {
+                for (int k = 0; k < TILE; k += 2) {
+                    const f32x2 x = pair(s[k], s[k + 1]), u = mul2(x, x);
+                    f32x2 h = fma2(u, pair(cap_low[3]), pair(cap_low[2]));
+                    h = fma2(h, u, pair(cap_low[1]));
+                    h = fma2(h, u, pair(cap_low[0]));
+                    const float2 y = both(mul2(x, h));
+                    s[k] = y.x;
+                    s[k + 1] = y.y;
+                }
+            } else if (__all_sync(0xffffffffu, far * to_cap <= 1.f)) {
 #pragma unroll
                 for (int k = 0; k < TILE; k += 2) {
                     const f32x2 x = pair(s[k], s[k + 1]);
@@ -738,6 +752,11 @@ __device__ void run_softmax(const Params& p, uint8_t* smem, uint32_t tmem, const
                     s[k] = y.x;
                     s[k + 1] = y.y;
                 }
+            } else {
+                const float in = 2.f * LOG2E * to_cap, out = p.softcap * LOG2E;
+#pragma unroll
+                for (int k = 0; k < TILE; ++k)
+                    s[k] = fmaf(-2.f * out, __fdividef(1.f, 1.f + ex2(s[k] * in)), out);
             }
         }
         if (kMode & 2) {
