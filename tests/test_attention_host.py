@@ -331,3 +331,92 @@ def test_append_units_cover_every_block():
                     b = mid
             assert unit_base(cu[a], a) <= unit
             assert a == len(news) - 1 or unit < unit_base(cu[a + 1], a + 1)
+
+
+# ------------------------------------------------------------------ decode dealing
+def pair_cost(n):
+    return 0 if n <= 0 else 1 + 2 * (n // 64) + (4 if n % 64 else 0)
+
+
+def block_start(b):
+    return 0 if b == 0 else 1 + 2 * b
+
+
+def blocks_before(x):
+    return 0 if x <= 0 else 1 if x <= 3 else x // 2
+
+
+def test_blocks_before_counts_the_starts():
+    starts = [block_start(b) for b in range(400)]
+    assert all(b - a <= 3 for a, b in zip(starts, starts[1:]))
+    for x in range(300):
+        assert blocks_before(x) == sum(s < x for s in starts)
+
+
+def test_decode_deals_every_block_once():
+    """The split's arithmetic, restated: every block of every (sequence, pair) goes to one warp,
+    a warp has at most one partial of each kind, and the join finds them where they are."""
+    rng = random.Random(1)
+    for _ in range(400):
+        seqs, pairs = rng.choice([1, 2, 3, 10, 50, 200]), rng.choice([1, 2, 8])
+        workers = rng.choice([8, 64, 1184])
+        lens = [rng.choice([0, 0, 1, 63, 64, 65, 100, 1000, rng.randrange(8000)])
+                for _ in range(seqs)]
+        first = [0]
+        for n in lens:
+            first.append(first[-1] + pair_cost(n) * pairs)
+        aligned = seqs * pairs <= workers // 4
+        over = workers - seqs * pairs if aligned else workers
+        share = max(-(-first[-1] // over), 3)
+        unit = [0]
+        for n in lens:
+            nb = -(-n // 64)
+            unit.append(unit[-1] + ((block_start(nb - 1) // share + 1) * pairs if nb else 0))
+        assert not aligned or unit[-1] <= workers
+        got, partial = {}, {}
+        for w in range(workers):
+            if aligned:
+                if w >= unit[-1]:
+                    continue
+                i = max(k for k in range(seqs) if unit[k] <= w)
+                per = block_start(-(-lens[i] // 64) - 1) // share + 1
+                pair, part = divmod(w - unit[i], per)
+                at = first[i] + pair * pair_cost(lens[i]) + part * share
+                end = min(at + share, first[i] + (pair + 1) * pair_cost(lens[i]))
+            else:
+                at = w * share
+                if at >= first[-1]:
+                    continue
+                end = min(at + share, first[-1])
+                i = max(k for k in range(seqs) if first[k] <= at)
+            while at < end:
+                while first[i + 1] <= at:
+                    i += 1
+                nb, cost = -(-lens[i] // 64), pair_cost(lens[i])
+                pair = (at - first[i]) // cost
+                base = first[i] + pair * cost
+                b0, b1 = blocks_before(at - base), min(nb, blocks_before(end - base))
+                at = base + cost
+                for b in range(b0, b1):
+                    assert (i, pair, b) not in got
+                    got[i, pair, b] = w
+                if b0 < b1 and b1 - b0 < nb:
+                    assert (w, b0 == 0) not in partial
+                    partial[w, b0 == 0] = i, pair
+        assert len(got) == sum(-(-n // 64) for n in lens) * pairs
+        for i, n in enumerate(lens):
+            if n == 0:
+                continue
+            last = block_start(-(-n // 64) - 1)
+            for pair in range(pairs):
+                if aligned:
+                    per = last // share + 1
+                    c0 = unit[i] + pair * per
+                    c1 = c0 + per
+                else:
+                    base = first[i] + pair_cost(n) * pair
+                    c0, c1 = base // share, (base + last) // share + 1
+                if c1 - c0 == 1:
+                    assert got[i, pair, 0] == got[i, pair, -(-n // 64) - 1] == c0
+                else:
+                    assert all(partial[c, c == c0] == (i, pair) for c in range(c0, c1))

@@ -31,7 +31,7 @@ def contexts():
 
 
 def ints(x):
-    return torch.tensor(x, dtype=torch.int32, device="cuda")
+    return torch.tensor(list(x), dtype=torch.int32, device="cuda")
 
 
 def rows(gen, n, heads, gain=1.0):
@@ -122,6 +122,24 @@ def test_append_ragged_batches(contexts):
                             cu_seqlens=ints(cu))
     ctx.check()
     assert_holds(cache, reference, slots)
+
+
+@pytest.mark.parametrize("count", [31, 32, 33, 64, 100, 1025])
+def test_append_many_sequences(contexts, count):
+    """The search of a work unit's sequence over more of them than a warp looks at at once."""
+    ctx = contexts(4, 1)
+    gen = generator(count)
+    cache, reference = fresh(ctx, max_seqs=count, max_blocks=2), ReferenceCache(1)
+    news = [(37 * i * i) % 90 for i in range(count)]
+    cu = [0]
+    for n in news:
+        cu.append(cu[-1] + n)
+    k, v = rows(gen, cu[-1] + 3, 1), rows(gen, cu[-1] + 3, 1)
+    ctx.kv_cache_append(cache, k, v, ints(range(count)), ints(news), cu_seqlens=ints(cu))
+    ctx.check()
+    for i in range(count):
+        reference.append(i, k[cu[i]:cu[i + 1]], v[cu[i]:cu[i + 1]])
+    assert_holds(cache, reference, range(count))
 
 
 def test_append_single_tokens(contexts):
