@@ -455,6 +455,14 @@ kvcache_append = _kvcache_append if _fast is None else _fast.kvcache_append
 kvcache_attention = _kvcache_attention if _fast is None else _fast.kvcache_attention
 
 
+# The same calls with tensors, where torch offers DLPack's C exchange API: they
+# return False without having done anything if an argument does not fit.
+_tensors = _fast is not None and _fast.use_exchange(torch.Tensor)
+try_attention = _fast.try_attention if _tensors else None
+try_append = _fast.try_append if _tensors else None
+try_decode = _fast.try_decode if _tensors else None
+
+
 def kvcache_attention_workspace(device, q_heads, kv_heads, seqs):
     return int(lib.fu_kvcache_attention_workspace(device, q_heads, kv_heads, seqs))
 

@@ -353,6 +353,14 @@ class FlashUlyssesContext:
                 -1 if index is None else index)
 
     @functools.cached_property
+    def _head_counts(self):
+        return self.output_q_heads, self.output_kv_heads
+
+    @functools.cached_property
+    def _default_scale(self):
+        return self.head_dim ** -0.5
+
+    @functools.cached_property
     def _attention_scratch(self):
         """Bytes of the decode attention's scratch."""
         return _C.kvcache_attention_workspace(self._widths[2], self.output_q_heads,
@@ -404,6 +412,14 @@ class FlashUlyssesContext:
         Lengths are read on the device, so a captured call may be replayed
         with other lengths in the same tensors.
         """
+        if _C.try_attention is not None and self._widths[2] >= 0:
+            to = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+            if _C.try_attention(self._widths[2], *self._head_counts, q, k, v, cu_seqlens,
+                                prefix_lens, alibi_slopes, to, causal,
+                                self._default_scale if scale is None else scale, softcap,
+                                self._status.device_ptr, self._status.host_ptr):
+                return to
+        # What did not fit, and what there is nothing to launch for.
         rows = q.shape[0]
         q_width, kv_width, index = self._widths
         q_ptr, q_stride = _rows("q", q, rows, q_width, index)
@@ -464,11 +480,16 @@ class FlashUlyssesContext:
         like every device-side error, by the next call or ``check()``, and
         nothing is written for them.
         """
+        _check_cache(cache, self._widths[1], self.device)
+        if _C.try_append is not None and self._widths[2] >= 0:
+            if _C.try_append(cache._address, k, v, slots, seq_lens, cu_seqlens,
+                             self._status.device_ptr, self._status.host_ptr):
+                return
+        # What did not fit, and what there is nothing to launch for.
         rows, count = k.shape[0], slots.numel()
         _, kv_width, index = self._widths
         k_ptr, k_stride = _rows("k", k, rows, kv_width, index)
         v_ptr, v_stride = _rows("v", v, rows, kv_width, index)
-        _check_cache(cache, kv_width, self.device)
         if rows > 1 << 30 or count > 1 << 24:
             raise ValueError("at most 2^30 rows and 2^24 sequences")
         slot_ptr = _vector("slots", slots, torch.int32, rows if cu_seqlens is None else count,
@@ -498,10 +519,22 @@ class FlashUlyssesContext:
         slot may occur more than once.  Slots, blocks and lengths that do not
         fit the cache are reported by the next call or ``check()``.
         """
+        _check_cache(cache, self._widths[1], self.device)
+        # Scratch from torch's allocator, so calls on other streams and captured
+        # graphs each have their own.
+        nbytes = self._attention_scratch
+        if _C.try_decode is not None and self._widths[2] >= 0:
+            to = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+            work = q.new_empty((nbytes + 1) // 2)
+            if _C.try_decode(cache._address, self._head_counts[0], q, slots, seq_lens,
+                             alibi_slopes, to, work,
+                             self._default_scale if scale is None else scale, softcap,
+                             self._status.device_ptr, self._status.host_ptr):
+                return to
+        # What did not fit, and what there is nothing to launch for.
         rows = q.shape[0]
         q_width, kv_width, index = self._widths
         q_ptr, q_stride = _rows("q", q, rows, q_width, index)
-        _check_cache(cache, kv_width, self.device)
         if rows > 1 << 24:
             raise ValueError("at most 2^24 sequences")
         slot_ptr = _vector("slots", slots, torch.int32, rows, index)
@@ -516,9 +549,6 @@ class FlashUlyssesContext:
             _no_overlap(rows, out_ptr, out_stride, q_width, q_ptr, q_stride, q_width)
         if rows == 0:
             return out
-        # Scratch from torch's allocator, so calls on other streams and captured
-        # graphs each have their own.
-        nbytes = self._attention_scratch
         work = q.new_empty((nbytes + 1) // 2)
         _C.kvcache_attention(cache._address, q_ptr, q_stride, out_ptr, out_stride,
                              self.output_q_heads, slot_ptr, lens_ptr, rows, scale, softcap,

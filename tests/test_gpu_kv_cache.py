@@ -264,6 +264,16 @@ def test_decode_scores(contexts, softcap, alibi, gain):
     check_decode(ctx, cache, reference, slots, lens, 8, 2, softcap=softcap, gain=gain, **options)
 
 
+@pytest.mark.parametrize("max_blocks", [1, 2, 4, 5])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (17, 1)])
+def test_decode_short_tables(contexts, max_blocks, q_heads, kv_heads):
+    """Tables of up to four blocks are not split over warps, longer ones are."""
+    ctx = contexts(q_heads, kv_heads)
+    lens = [64 * max_blocks, 64 * max_blocks - 1, 1, 63, 0, 64 * max_blocks - 63]
+    cache, reference, slots = filled(ctx, lens, kv_heads, max_blocks=max_blocks)
+    check_decode(ctx, cache, reference, slots, lens, q_heads, kv_heads)
+
+
 def test_decode_many_sequences(contexts):
     ctx = contexts(8, 2)
     lens = [(37 * i * i + 11) % 500 for i in range(300)]

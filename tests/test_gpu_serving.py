@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from attention_reference import DIM, ReferenceCache, assert_close, attention, decode
-from flash_ulysses_b200 import FlashUlyssesContext
+from flash_ulysses_b200 import FlashUlyssesContext, _C
 from flash_ulysses_b200.workloads import make_parameters
 
 pytestmark = pytest.mark.gpu
@@ -92,5 +92,68 @@ def test_decode_equals_the_last_row_of_the_prompt():
         want, size = attention(q, k, v, HQ, HKV)
         assert_close(prompt[62:], want[62:], size[62:])
         assert_close(last, want[62:], size[62:])
+    finally:
+        ctx.close()
+
+
+def test_both_ways_of_calling(monkeypatch):
+    """Tensors are read in C where they fit and in Python where not: the same bits, and the same
+    refusals."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    ctx = FlashUlyssesContext(rank=0, world_size=1, max_local_tokens=1, hidden_size=64,
+                              num_heads=HQ, num_kv_heads=HKV, sp_size=1)
+    assert _C.try_attention is not None
+    try:
+        def rows(n, h):
+            return torch.randn(n, h * DIM, generator=gen, device="cuda").bfloat16()
+
+        q, k, v, one = rows(200, HQ), rows(200, HKV), rows(200, HKV), rows(1, HQ)
+        cu, pre = ints([0, 90, 200]), ints([20, 0])
+        slopes = torch.rand(HQ, generator=gen, device="cuda")
+        slot, length = ints([0]), ints([200])
+        caches = [ctx.create_kv_cache(4, 1, 4) for _ in range(2)]
+        got = []
+        for cache in caches:
+            cache.block_table.copy_(ints([[2, 0, 3, 1]]))
+            ctx.kv_cache_append(cache, k, v, slot, length, cu_seqlens=ints([0, 200]))
+            got.append((
+                ctx.ulysses_attention_forward(q, k, v, cu_seqlens=cu, prefix_lens=pre, softcap=20,
+                                              alibi_slopes=slopes, scale=0.1),
+                ctx.kv_cache_attention(cache, one, slot, length, alibi_slopes=slopes),
+                cache.k_blocks.view(torch.uint8), cache.v_tail))
+            for name in ("try_attention", "try_append", "try_decode"):
+                monkeypatch.setattr(_C, name, None)
+        ctx.check()
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+        monkeypatch.undo()
+
+        cache, i64 = caches[0], slot.long()
+        for call in (
+                lambda: ctx.ulysses_attention_forward(q.float(), k, v),
+                lambda: ctx.ulysses_attention_forward(q, k[:199], v),
+                lambda: ctx.ulysses_attention_forward(q, k.cpu(), v),
+                lambda: ctx.ulysses_attention_forward(q, k, v, out=q),
+                lambda: ctx.ulysses_attention_forward(q, k, v, out=rows(199, HQ)),
+                lambda: ctx.ulysses_attention_forward(q, k, v, cu_seqlens=cu.long()),
+                lambda: ctx.ulysses_attention_forward(q, k, v, cu_seqlens=cu, prefix_lens=pre[:1]),
+                lambda: ctx.ulysses_attention_forward(q, k, v, prefix_lens=pre[:1], causal=False),
+                lambda: ctx.ulysses_attention_forward(q, k, v, alibi_slopes=slopes[:4]),
+                lambda: ctx.ulysses_attention_forward(q, k, v, softcap=-1.0),
+                lambda: ctx.ulysses_attention_forward(q, k, v, scale=float("nan")),
+                lambda: ctx.kv_cache_append(cache, k, v, slot, length),
+                lambda: ctx.kv_cache_append(cache, k[:1], v[:1], i64, length),
+                lambda: ctx.kv_cache_append(cache, k[:1], q[:1], slot, length),
+                lambda: ctx.kv_cache_attention(cache, one, slot, length.float()),
+                lambda: ctx.kv_cache_attention(cache, q, slot, length),
+                lambda: ctx.kv_cache_attention(cache, one, slot, length, out=one),
+                lambda: ctx.kv_cache_attention(cache, one.half(), slot, length)):
+            with pytest.raises(ValueError):
+                call()
+        # Tensors that take part in autograd, and their subclasses, are read like any other.
+        grad = torch.nn.Parameter(q)
+        for x in (grad, q.clone().requires_grad_()):
+            assert torch.equal(ctx.ulysses_attention_forward(x, k, v),
+                               ctx.ulysses_attention_forward(q, k, v))
+        ctx.check()
     finally:
         ctx.close()
