@@ -79,7 +79,8 @@ def _no_overlap(rows, out, out_stride, out_width, t, stride, width):
 
 
 def _check_cache(cache, kv_width, device):
-    if (cache.device is not device and cache.device != device) or cache.kv_heads * _C.FU_HEAD_DIM != kv_width:
+    if ((cache.device is not device and cache.device != device)
+            or cache.kv_heads * _C.FU_HEAD_DIM != kv_width):
         raise ValueError(f"the cache must hold {kv_width // _C.FU_HEAD_DIM} K/V heads on {device}")
 
 
@@ -369,8 +370,11 @@ class FlashUlyssesContext:
     def _score_options(self, scale, softcap, alibi_slopes):
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
         softcap = float(softcap)
-        if not math.isfinite(scale) or not math.isfinite(softcap) or softcap < 0:
-            raise ValueError("scale must be finite, softcap finite and not negative")
+        if not abs(scale) <= 1e30:
+            raise ValueError("scale must be within -1e30 and 1e30")
+        if softcap != 0 and not (1e-3 <= softcap <= 1e6 and abs(scale) <= 1e9 * softcap):
+            raise ValueError("softcap must be 0, or within 1e-3 and 1e6 and no less than "
+                             "1e-9 times the scale")
         slopes = None
         if alibi_slopes is not None:
             slopes = _vector("alibi_slopes", alibi_slopes, torch.float32, self.output_q_heads,
@@ -396,7 +400,8 @@ class FlashUlyssesContext:
         into the rows: document ``d`` is rows ``cu_seqlens[d]`` up to
         ``cu_seqlens[d + 1]``, and a row sees rows of its own document only.
         It starts at 0 and does not decrease; rows behind its last entry are
-        neither read nor written.  Without it all rows are one document.
+        not written and have no part in others.  Without it all rows are one
+        document.
         ``causal=True`` lets a row see itself and the rows before it, and with
         ``prefix_lens`` (int32, ``[documents]``, needs ``causal``) also the
         first ``prefix_lens[d]`` rows of its document.
@@ -404,8 +409,10 @@ class FlashUlyssesContext:
         Scores are ``scale * q.k`` (default ``128 ** -0.5``), then
         ``softcap * tanh(score / softcap)`` if ``softcap`` is positive, then
         less ``alibi_slopes[h] * |i - j|`` if ``alibi_slopes`` (FP32
-        ``[output_q_heads]``, this rank's heads) is given.  Scores and sums are
-        FP32.  Rows that are not seen take no part, whatever they hold.
+        ``[output_q_heads]``, this rank's heads) is given.  A ``softcap`` lies
+        within 1e-3 and 1e6 and is at least ``1e-9 * abs(scale)``; ``scale`` lies
+        within -1e30 and 1e30.  Scores and sums are FP32.  Rows that are not
+        seen take no part, whatever they hold.
 
         Returns BF16 ``[T, output_q_heads * 128]``, the layout that
         ``ulysses_o_proj_forward`` takes, written into ``out`` when given.

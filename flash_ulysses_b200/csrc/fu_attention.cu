@@ -679,223 +679,242 @@ __device__ void run_softmax(const Params& p, uint8_t* smem, uint32_t tmem, const
     const float lin = p.scale * LOG2E;
     const float to_cap = kMode & 1 ? p.scale / p.softcap : 0.f;
     const float z2 = to_cap * to_cap;
-    // tanh(z) = z + .. to z^7 for |z| <= 1/2, off by 2e-7, as a polynomial in s (the last
-    // coefficient would underflow for a cap above some 10^4 times the scale's inverse).
+    // tanh(z) = z + .. to z^7 for |z| <= 1/2, off by 2e-7, as a polynomial in s, where
+    // its coefficients stay within FP32's range.
     const float cap_low[4] = {lin, -0.33326461911201477f * lin * z2,
                               0.13185861706733704f * lin * z2 * z2,
                               -0.04422929883003235f * lin * z2 * z2 * z2};
-    const bool cap_small = to_cap >= 1e-5f;
+    const bool cap_small = to_cap >= 1e-5f && to_cap <= 1e4f;
     const auto wait = [&](uint32_t bar, uint32_t parity, int where) -> bool {
         return __all_sync(0xffffffffu, fu_wait_parity(bar, parity, abort_flag, p.timeout_ns,
                                                       p.status, where));
     };
     uint32_t phase = 0, o_phase = 0;
     for (int n = 0;; ++n) {
-    const int slot = n % SLOTS;
-    if (!wait(b.item_full + 8 * slot, (n / SLOTS) & 1, W_ITEM)) return;
-    const Item& w = *reinterpret_cast<const Item*>(smem + OFF_ITEM + 64 * slot);
-    if (w.tiles < 0) return;
-    const int first = w.first[t], last = w.last[t], kv0 = w.kv0;
-    const int row = w.row0 + t * TILE + warp * 32 + lane;
-    const float slope = kMode & 2 ? __ldg(p.alibi_slopes + w.head) * LOG2E : 0.f;
-    const int2 seen = row < p.tokens ? seen_rows(p, row) : make_int2(0, 0);
-    const bool valid = seen.x < seen.y;
-    // A row without a document is computed like one that sees everything, and
-    // not stored.
-    const int lo = valid ? seen.x : INT_MIN / 2, hi = valid ? seen.y : INT_MAX / 2;
+        const int slot = n % SLOTS;
+        if (!wait(b.item_full + 8 * slot, (n / SLOTS) & 1, W_ITEM)) return;
+        const Item& w = *reinterpret_cast<const Item*>(smem + OFF_ITEM + 64 * slot);
+        if (w.tiles < 0) return;
+        const int first = w.first[t], last = w.last[t], kv0 = w.kv0;
+        const int row = w.row0 + t * TILE + warp * 32 + lane;
+        const float slope = kMode & 2 ? __ldg(p.alibi_slopes + w.head) * LOG2E : 0.f;
+        const int2 seen = row < p.tokens ? seen_rows(p, row) : make_int2(0, 0);
+        const bool valid = seen.x < seen.y;
+        // A row without a document is computed like one that sees everything, and
+        // not stored.
+        const int lo = valid ? seen.x : INT_MIN / 2, hi = valid ? seen.y : INT_MAX / 2;
 
-    float m = -INFINITY, l = 0.f;
-    for (int j = first; j < last; ++j) {
-        if (!wait(b.s + 8 * t, phase, W_S)) return;
-        phase ^= 1;
-        tc_fence_after();
-        uint32_t r[TILE];
-        float* s = reinterpret_cast<float*>(r);
+        float m = -INFINITY, l = 0.f;
+        for (int j = first; j < last; ++j) {
+            if (!wait(b.s + 8 * t, phase, W_S)) return;
+            phase ^= 1;
+            tc_fence_after();
+            uint32_t r[TILE];
+            float* s = reinterpret_cast<float*>(r);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            tmem_ld_32cols(tm_s + 32 * k, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * k));
-        tmem_ld_wait();
-        const int k0 = kv0 + j * TILE;
-        if (kMode & 1) {
-            // cap tanh(z), z = scale s / cap.  Where all of the warp's |z| are at most
-            // 1/2 (scores well below the cap, the ordinary case) by an odd polynomial
-            // of degree 7, at most 1 by one of degree 11, off by 7e-7; else as
-            // cap (1 - 2 / (1 + 2^(2 log2(e) z))), off by 2^-22: absolute errors in all,
-            // which is what a score needs.  A packed FMA takes its pipe two clocks, so
-            // the polynomials' length is what a cap costs; the last form takes three
-            // special-function results per score with the weight's.
-            float far = 0.f;
-#pragma unroll
-            for (int k = 0; k < TILE; k += 2) far = max3(far, fabsf(s[k]), fabsf(s[k + 1]));
-            if (__all_sync(0xffffffffu, cap_small && far * to_cap <= 0.5f)) {
-#pragma unroll
-                for (int k = 0; k < TILE; k += 2) {
-                    const f32x2 x = pair(s[k], s[k + 1]), u = mul2(x, x);
-                    f32x2 h = fma2(u, pair(cap_low[3]), pair(cap_low[2]));
-                    h = fma2(h, u, pair(cap_low[1]));
-                    h = fma2(h, u, pair(cap_low[0]));
-                    const float2 y = both(mul2(x, h));
-                    s[k] = y.x;
-                    s[k + 1] = y.y;
-                }
-            } else if (__all_sync(0xffffffffu, far * to_cap <= 1.f)) {
-#pragma unroll
-                for (int k = 0; k < TILE; k += 2) {
-                    const f32x2 x = pair(s[k], s[k + 1]);
-                    const f32x2 z = mul2(x, pair(to_cap)), u = mul2(z, z);
+            for (int k = 0; k < 4; ++k)
+                tmem_ld_32cols(tm_s + 32 * k, *reinterpret_cast<uint32_t(*)[32]>(r + 32 * k));
+            tmem_ld_wait();
+            const int k0 = kv0 + j * TILE;
+            if (kMode & 1) {
+                // cap tanh(z), z = scale s / cap.  Where all of the warp's |z| are at most
+                // 1/2 (scores well below the cap, the ordinary case) by an odd polynomial
+                // of degree 7, at most 1 by one of degree 11, off by 7e-7 with the slope at 0
+                // exact; else as cap (1 - 2 / (1 + 2^(2 log2(e) z))), off by 2^-22.  Times the
+                // cap these are absolute errors, which for a cap above FINE matter for scores
+                // far below it: there the last form takes the polynomial for |z| <= 1, and
+                // a score is off by 2^-20 of itself.  A packed FMA takes its pipe two clocks, so
+                // the polynomials' length is what a cap costs; the last form takes three
+                // special-function results per score with the weight's.
+                constexpr float FINE = 1024.f;
+                const f32x2 to_cap2 = pair(to_cap), lin2 = pair(lin);
+                const auto degree_11 = [&](f32x2 x) {
+                    const f32x2 z = mul2(x, to_cap2), u = mul2(z, z);
                     f32x2 h = fma2(u, pair(-0.0030804092530161142f), pair(0.016842123121023178f));
                     h = fma2(h, u, pair(-0.051767539232969284f));
                     h = fma2(h, u, pair(0.1329089254140854f));
                     h = fma2(h, u, pair(-0.3333089351654053f));
                     h = fma2(h, u, pair(1.f));
-                    const float2 y = both(mul2(mul2(x, pair(lin)), h));
-                    s[k] = y.x;
-                    s[k + 1] = y.y;
-                }
-            } else {
-                const float in = 2.f * LOG2E * to_cap, out = p.softcap * LOG2E;
+                    return both(mul2(mul2(x, lin2), h));
+                };
+                float far = 0.f;
 #pragma unroll
-                for (int k = 0; k < TILE; ++k)
-                    s[k] = fmaf(-2.f * out, __fdividef(1.f, 1.f + ex2(s[k] * in)), out);
-            }
-        }
-        if (kMode & 2) {
-            const f32x2 scale2 = pair(kMode & 1 ? 1.f : lin);
-            // Without keys behind the row (or with only such) |i - j| is linear in
-            // j; keys that a causal mask hides may come out as they like.
-            const bool below = (p.causal && p.prefix_lens == nullptr) || k0 + TILE - 1 <= row - lane;
-            const bool above = k0 >= row - lane + 31;
-            if (below || above) {
-                const float step = below ? slope : -slope;
+                for (int k = 0; k < TILE; k += 2) far = max3(far, fabsf(s[k]), fabsf(s[k + 1]));
+                if (__all_sync(0xffffffffu, cap_small && far * to_cap <= 0.5f)) {
 #pragma unroll
-                for (int k = 0; k < TILE; k += 32) {
-                    const float start = static_cast<float>(k0 + k - row) * step;
-                    f32x2 bias = pair(start, start + step);
+                    for (int k = 0; k < TILE; k += 2) {
+                        const f32x2 x = pair(s[k], s[k + 1]), u = mul2(x, x);
+                        f32x2 h = fma2(u, pair(cap_low[3]), pair(cap_low[2]));
+                        h = fma2(h, u, pair(cap_low[1]));
+                        h = fma2(h, u, pair(cap_low[0]));
+                        const float2 y = both(mul2(x, h));
+                        s[k] = y.x;
+                        s[k + 1] = y.y;
+                    }
+                } else if (__all_sync(0xffffffffu, far * to_cap <= 1.f)) {
 #pragma unroll
-                    for (int q = k; q < k + 32; q += 2) {
-                        const float2 y = both(fma2(pair(s[q], s[q + 1]), scale2, bias));
-                        s[q] = y.x;
-                        s[q + 1] = y.y;
-                        bias = add2(bias, pair(2.f * step));
+                    for (int k = 0; k < TILE; k += 2) {
+                        const float2 y = degree_11(pair(s[k], s[k + 1]));
+                        s[k] = y.x;
+                        s[k + 1] = y.y;
+                    }
+                } else {
+                    const float in = 2.f * LOG2E * to_cap, out = p.softcap * LOG2E;
+                    const auto full = [&](float x) {
+                        return fmaf(-2.f * out, __fdividef(1.f, 1.f + ex2(x * in)), out);
+                    };
+                    if (p.softcap <= FINE) {
+#pragma unroll
+                        for (int k = 0; k < TILE; ++k) s[k] = full(s[k]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < TILE; k += 2) {
+                            const float2 y = degree_11(pair(s[k], s[k + 1]));
+                            s[k] = fabsf(s[k] * to_cap) <= 1.f ? y.x : full(s[k]);
+                            s[k + 1] = fabsf(s[k + 1] * to_cap) <= 1.f ? y.y : full(s[k + 1]);
+                        }
                     }
                 }
-            } else {
-                const float at = static_cast<float>(row - k0);
+            }
+            if (kMode & 2) {
+                const f32x2 scale2 = pair(kMode & 1 ? 1.f : lin);
+                // Without keys behind the row (or with only such) |i - j| is linear in
+                // j; keys that a causal mask hides may come out as they like.
+                const bool below = (p.causal && p.prefix_lens == nullptr) ||
+                                   k0 + TILE - 1 <= row - lane;
+                const bool above = k0 >= row - lane + 31;
+                if (below || above) {
+                    const float step = below ? slope : -slope;
+#pragma unroll
+                    for (int k = 0; k < TILE; k += 32) {
+                        const float start = static_cast<float>(k0 + k - row) * step;
+                        f32x2 bias = pair(start, start + step);
+#pragma unroll
+                        for (int q = k; q < k + 32; q += 2) {
+                            const float2 y = both(fma2(pair(s[q], s[q + 1]), scale2, bias));
+                            s[q] = y.x;
+                            s[q + 1] = y.y;
+                            bias = add2(bias, pair(2.f * step));
+                        }
+                    }
+                } else {
+                    const float at = static_cast<float>(row - k0);
+#pragma unroll
+                    for (int k = 0; k < TILE; ++k)
+                        s[k] = fmaf(-slope, fabsf(at - static_cast<float>(k)),
+                                    kMode & 1 ? s[k] : s[k] * lin);
+                }
+            }
+            const int from = lo - k0, to = hi - k0;
+            if (__any_sync(0xffffffffu, from > 0 || to < TILE)) {
 #pragma unroll
                 for (int k = 0; k < TILE; ++k)
-                    s[k] = fmaf(-slope, fabsf(at - static_cast<float>(k)),
-                                kMode & 1 ? s[k] : s[k] * lin);
+                    s[k] = k >= from && k < to ? s[k] : -INFINITY;
             }
-        }
-        const int from = lo - k0, to = hi - k0;
-        if (__any_sync(0xffffffffu, from > 0 || to < TILE)) {
+            float best[4] = {m, s[0], s[1], s[2]};
 #pragma unroll
-            for (int k = 0; k < TILE; ++k)
-                s[k] = k >= from && k < to ? s[k] : -INFINITY;
-        }
-        float best[4] = {m, s[0], s[1], s[2]};
+            for (int k = 3; k + 1 < TILE; k += 2)
+                best[(k >> 1) & 3] = max3(best[(k >> 1) & 3], s[k], s[k + 1]);
+            const float top = fmaxf(max3(best[0], best[1], best[2]), fmaxf(best[3], s[TILE - 1]));
+            if (j == first) {
+                m = top;
+            } else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
+                const float f = top == -INFINITY ? 1.f : ex2((m - top) * c);
+                l *= f;
+                m = top;
+#pragma unroll 1
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t o[32];
+                    tmem_ld_32cols(tm_o + 32 * k, o);
+                    tmem_ld_wait();
 #pragma unroll
-        for (int k = 3; k + 1 < TILE; k += 2)
-            best[(k >> 1) & 3] = max3(best[(k >> 1) & 3], s[k], s[k + 1]);
-        const float top = fmaxf(max3(best[0], best[1], best[2]), fmaxf(best[3], s[TILE - 1]));
-        if (j == first) {
-            m = top;
-        } else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) {
-            const float f = top == -INFINITY ? 1.f : ex2((m - top) * c);
-            l *= f;
-            m = top;
+                    for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+                    tmem_st_32cols(tm_o + 32 * k, o);
+                }
+            }
+            const f32x2 base = pair(m == -INFINITY ? 0.f : -m * c), c2 = pair(c);
+            f32x2 sum[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    const f32x2 x = pair(s[32 * k + 2 * q], s[32 * k + 2 * q + 1]);
+                    f32x2 y = kMode ? add2(x, base) : fma2(x, c2, base);
+                    if (!(kMode & 1) && q % POLY_EVERY == POLY_EVERY - 1) {
+                        y = ex2_poly(y);
+                    } else {
+                        const float2 z = both(y);
+                        y = pair(ex2(z.x), ex2(z.y));
+                    }
+                    sum[q & 3] = add2(sum[q & 3], y);
+                    const float2 z = both(y);
+                    packed[q] = pack_bf16x2_rn(z.x, z.y);
+                }
+                tmem_st_16cols(tm_s + 16 * k, packed);
+                if (k & 1) {
+                    // Half of P is there: the product may begin.
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(b.p + 16 * t + 8 * (k >> 1));
+                }
+            }
+            const float2 total = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+            l += total.x + total.y;
+        }
+        if (first < last) {
+            // out = O / l, a row of 256 bytes a thread.
+            if (!wait(b.o + 8 * t, o_phase, W_O)) return;
+            o_phase ^= 1;
+            tc_fence_after();
+            const float inv = 1.f / l;
+            const bool poison = *const_cast<const volatile int*>(&w.found) != 0;
+            __nv_bfloat16* dst = p.out + static_cast<int64_t>(row) * p.out_stride + w.head * D;
 #pragma unroll 1
             for (int k = 0; k < 4; ++k) {
                 uint32_t o[32];
                 tmem_ld_32cols(tm_o + 32 * k, o);
                 tmem_ld_wait();
 #pragma unroll
-                for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
-                tmem_st_32cols(tm_o + 32 * k, o);
-            }
-        }
-        const f32x2 base = pair(m == -INFINITY ? 0.f : -m * c), c2 = pair(c);
-        f32x2 sum[4] = {0, 0, 0, 0};
+                for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * inv);
+                if (poison && valid) {
+                    // What run_clean() took out, for the rows that see it.
+                    for (int j = first; j < last; ++j) {
+                        if (!w.edge(j)) continue;
+                        const int a = max(lo, kv0 + j * TILE), e = min(hi, kv0 + (j + 1) * TILE);
+                        for (int key = a; key < e; ++key) {
+                            const __nv_bfloat16* v =
+                                p.v + key * p.v_stride + w.head / p.group * D + 32 * k;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            uint32_t packed[16];
-#pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const f32x2 x = pair(s[32 * k + 2 * q], s[32 * k + 2 * q + 1]);
-                f32x2 y = kMode ? add2(x, base) : fma2(x, c2, base);
-                if (!(kMode & 1) && q % POLY_EVERY == POLY_EVERY - 1) {
-                    y = ex2_poly(y);
-                } else {
-                    const float2 z = both(y);
-                    y = pair(ex2(z.x), ex2(z.y));
-                }
-                sum[q & 3] = add2(sum[q & 3], y);
-                const float2 z = both(y);
-                packed[q] = pack_bf16x2_rn(z.x, z.y);
-            }
-            tmem_st_16cols(tm_s + 16 * k, packed);
-            if (k & 1) {
-                // Half of P is there: the product may begin.
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b.p + 16 * t + 8 * (k >> 1));
-            }
-        }
-        const float2 total = both(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-        l += total.x + total.y;
-    }
-    if (first < last) {
-        // out = O / l, a row of 256 bytes a thread.
-        if (!wait(b.o + 8 * t, o_phase, W_O)) return;
-        o_phase ^= 1;
-        tc_fence_after();
-        const float inv = 1.f / l;
-        const bool poison = *const_cast<const volatile int*>(&w.found) != 0;
-        __nv_bfloat16* dst = p.out + static_cast<int64_t>(row) * p.out_stride + w.head * D;
-#pragma unroll 1
-        for (int k = 0; k < 4; ++k) {
-            uint32_t o[32];
-            tmem_ld_32cols(tm_o + 32 * k, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * inv);
-            if (poison && valid) {
-                // What run_clean() took out, for the rows that see it.
-                for (int j = first; j < last; ++j) {
-                    if (!w.edge(j)) continue;
-                    const int a = max(lo, kv0 + j * TILE), e = min(hi, kv0 + (j + 1) * TILE);
-                    for (int key = a; key < e; ++key) {
-                        const __nv_bfloat16* v =
-                            p.v + key * p.v_stride + w.head / p.group * D + 32 * k;
-#pragma unroll
-                        for (int q = 0; q < 32; ++q) {
-                            const float x = __bfloat162float(v[q]);
-                            if (!isfinite(x)) o[q] = __float_as_uint(__uint_as_float(o[q]) + x);
+                            for (int q = 0; q < 32; ++q) {
+                                const float x = __bfloat162float(v[q]);
+                                if (!isfinite(x)) o[q] = __float_as_uint(__uint_as_float(o[q]) + x);
+                            }
                         }
                     }
                 }
-            }
-            uint32_t packed[16];
+                uint32_t packed[16];
 #pragma unroll
-            for (int q = 0; q < 16; ++q)
-                packed[q] = pack_bf16x2_rn(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1]));
-            if (!valid) continue;
-            if (p.wide_store) {
-                store_32_bytes(dst + 32 * k, packed);
-                store_32_bytes(dst + 32 * k + 16, packed + 8);
-            } else {
+                for (int q = 0; q < 16; ++q)
+                    packed[q] =
+                        pack_bf16x2_rn(__uint_as_float(o[2 * q]), __uint_as_float(o[2 * q + 1]));
+                if (!valid) continue;
+                if (p.wide_store) {
+                    store_32_bytes(dst + 32 * k, packed);
+                    store_32_bytes(dst + 32 * k + 16, packed + 8);
+                } else {
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<uint4*>(dst + 32 * k + 8 * q) = make_uint4(
-                        packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<uint4*>(dst + 32 * k + 8 * q) = make_uint4(
+                            packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+                }
             }
+            // The next product into O comes behind weights of these warps.
+            tc_fence_before();
         }
-        // The next product into O comes behind weights of these warps.
-        tc_fence_before();
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(b.item_empty + 8 * slot);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b.item_empty + 8 * slot);
     }
 }
 
@@ -1062,8 +1081,8 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
         return set_error(FU_ERR_INVALID, "docs %d does not go with cu_seqlens", a->docs);
     if (a->prefix_lens != nullptr && !a->causal)
         return set_error(FU_ERR_INVALID, "prefix_lens need a causal mask");
-    if (!(a->softcap >= 0.f) || !std::isfinite(a->softcap) || !std::isfinite(a->scale))
-        return set_error(FU_ERR_INVALID, "scale must be finite, softcap finite and 0 or more");
+    int rc = check_scores(a->scale, a->softcap);
+    if (rc != FU_OK) return rc;
     if (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->out == nullptr)
         return set_error(FU_ERR_INVALID, "null tensor argument");
     const struct { const void* ptr; int64_t stride; int heads; const char* name; } rows[4] = {
@@ -1085,8 +1104,8 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
         return set_error(FU_ERR_INVALID, "tokens * q_heads is too large for one call");
 
     attention::Params p = {};
-    int rc = attention::encode_rows(&p.tm_q, a->q, a->tokens, a->q_heads * attention::D,
-                                    a->q_stride, "q");
+    rc = attention::encode_rows(&p.tm_q, a->q, a->tokens, a->q_heads * attention::D, a->q_stride,
+                                "q");
     if (rc == FU_OK)
         rc = attention::encode_rows(&p.tm_k, a->k, a->tokens, a->kv_heads * attention::D,
                                     a->k_stride, "k");

@@ -17,6 +17,17 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiledFn encode_tiled_fn();
 
+// The range within which no factor of an attention score leaves FP32's (a softcap of
+// 10^-30 would make an infinity of scale / softcap, and NaN of a score of 0).
+inline int check_scores(float scale, float softcap) {
+    const float size = scale < 0.f ? -scale : scale;
+    if (!(size <= 1e30f)) return set_error(1, "scale must be within -1e30 and 1e30");
+    if (softcap != 0.f && !(softcap >= 1e-3f && softcap <= 1e6f && size <= 1e9f * softcap))
+        return set_error(1, "softcap must be 0, or within 1e-3 and 1e6 and no less than "
+                            "1e-9 times the scale");
+    return 0;
+}
+
 // Makes `device` current for a scope.
 struct DeviceGuard {
     int prev = -1;

@@ -128,8 +128,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
     bool again = false;
     for (int o = threadIdx.x; o < i; o += APPEND_THREADS) again |= __ldg(p.slots + o) == slot;
 
-    const __nv_bfloat16* rows = p.rows[which] + static_cast<int64_t>(row0) * p.stride[which] + h * D;
     const int64_t stride = p.stride[which];
+    const __nv_bfloat16* rows = p.rows[which] + row0 * stride + h * D;
     __nv_bfloat16* tail = p.tail[which] + (static_cast<int64_t>(slot) * p.kv_heads + h) * BLOCK * D;
     const int tg = t >> 4, c = t & 15;                 // token group (and tg + 8), 8-dim chunk
 
@@ -238,8 +238,8 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
     // block that stays unfinished (after the barriers above when it read it).
     if (j == 0) {
         const int first = max(full * BLOCK - start, 0);     // first row that goes to the tail
-        for (int o = first * 16 + t; o < n * 16; o += 128) {
-            const int r = o >> 4, at = (start + r) % BLOCK;
+        for (int o = t; o < (n - first) * 16; o += 128) {   // (fewer than 64 rows)
+            const int r = first + (o >> 4), at = (start + r) % BLOCK;
             *reinterpret_cast<uint4*>(tail + at * D + 8 * (o & 15)) =
                 *reinterpret_cast<const uint4*>(rows + r * stride + 8 * (o & 15));
         }
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 // weights as a sum of two BF16 so that they keep 16 bits.
 constexpr int WARPS = 4;
 constexpr int SPLIT_THREADS = 32 * WARPS;
-constexpr int MAX_BATCH = 1024;        // sequences per launch (their prefix sums sit in shared memory)
+constexpr int MAX_BATCH = 1024;        // sequences per launch (prefix sums in shared memory)
 constexpr int TILE_BYTES = BLOCK * D;  // one stage of a warp's ring: K or V of a block
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -429,15 +429,34 @@ struct Rows {
     }
 };
 
-// The score's path from the raw product to log2 units, and what it needs of a row.
+// A score's path from the product to log2 units, and what it needs of a row.  kMode: 1
+// capped by a tanh, 2 lowered with distance, 4 (with 1) by a cap above FINE.
+//
+// With x = 2 log2(e) z, cap tanh(z) = cap (1 - 2 / (1 + 2^x)) is off by 2^-22 cap: up to
+// a cap of FINE a small part of what rounding the weights to f16 costs.  Larger caps
+// matter for scores far below them, which take an odd polynomial of degree 7 in z, off
+// by 2e-7 with the slope at 0 exact: relative to the score it is off by 2^-21 whatever
+// the cap.  (Both forms in one kernel: 34.8 us instead of 33.5 us for 256 sequences of up to
+// 1500 tokens with the first.)
+constexpr float FINE = 256.f;
 template <int kMode>
 struct Score {
-    float factor, cap_out, slope;      // per row; with a cap `factor` is that of 2 log2(e) z
+    float factor, cap_out, slope;      // per row; with a cap `factor` is that of x
     __device__ float operator()(float raw, float block_scale, int distance) const {
         float x = raw * (factor * block_scale);
         if (kMode & 1) {
-            // cap tanh(z) = cap (1 - 2 / (1 + 2^(2 log2(e) z))): an absolute error of 2^-22 cap.
-            x = fmaf(-2.f * cap_out, __fdividef(1.f, 1.f + ex2(x)), cap_out);
+            const float far = fmaf(-2.f * cap_out, __fdividef(1.f, 1.f + ex2(x)), cap_out);
+            if (kMode & 4) {
+                constexpr float Z = 0.5f / LOG2E;              // z = Z x
+                const float u = x * x;
+                float near = fmaf(u, -0.04422929883003235f * Z * Z * Z * Z * Z * Z * Z,
+                                  0.13185861706733704f * Z * Z * Z * Z * Z);
+                near = fmaf(near, u, -0.33326461911201477f * Z * Z * Z);
+                near = fmaf(near, u, Z) * (x * cap_out);
+                x = fabsf(x) <= LOG2E ? near : far;            // |z| = 1/2
+            } else {
+                x = far;
+            }
         }
         if (kMode & 2) x = fmaf(-slope, static_cast<float>(distance), x);
         return x;
@@ -685,7 +704,7 @@ attention_split_kernel(const AttentionParams p) {
                 parts = 2 * halves;
                 const int part = sub % halves;
                 src = reinterpret_cast<const uint8_t*>(sub < halves ? p.k_tail : p.v_tail) +
-                      (static_cast<int64_t>(feed.slot) * p.kv_heads + feed.head) * (2 * TILE_BYTES) +
+                      (static_cast<int64_t>(feed.slot) * p.kv_heads + feed.head) * 2 * TILE_BYTES +
                       part * TILE_BYTES;
                 bytes = min(left - 32 * part, 32) * D * 2;
             }
@@ -758,7 +777,8 @@ attention_split_kernel(const AttentionParams p) {
                 for (int c = 0; c < 4; ++c) raw_q[h][c] = load_q(h, c);
                 score[h].slope =
                     (kMode & 2) && g + 8 * h < rows
-                        ? __ldg(p.alibi_slopes + walk.head * p.group + walk.row0 + g + 8 * h) * LOG2E
+                        ? __ldg(p.alibi_slopes + walk.head * p.group + walk.row0 + g + 8 * h) *
+                              LOG2E
                         : 0.f;
             }
         }
@@ -777,7 +797,7 @@ attention_split_kernel(const AttentionParams p) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // q = (q 2^-e) 2^e with the row's largest value in [1, 2).
-                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 100);
+                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -96), 96);
                 const float down = __int_as_float((127 - e) << 23);
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
@@ -803,7 +823,8 @@ attention_split_kernel(const AttentionParams p) {
                         uint4 x[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            x[j] = *reinterpret_cast<const uint4*>(tile + 2 * (j0 + j) * D + 64 * y);
+                            x[j] = *reinterpret_cast<const uint4*>(tile + 2 * (j0 + j) * D +
+                                                                   64 * y);
 #pragma unroll
                         for (int k = 4 * y; k < 4 * y + 4; ++k)
 #pragma unroll
@@ -887,8 +908,10 @@ attention_split_kernel(const AttentionParams p) {
                                                           8 * (c & 1)) * 2)
                                             : make_uint4(0, 0, 0, 0);
                         const uint4 q0 = qb[0][c], q1 = qb[H - 1][c];
-                        mma_bf16(acc, Words{{q0.x, kWide ? q1.x : 0u, q0.y, kWide ? q1.y : 0u}}, x.x, x.y);
-                        mma_bf16(acc, Words{{q0.z, kWide ? q1.z : 0u, q0.w, kWide ? q1.w : 0u}}, x.z, x.w);
+                        mma_bf16(acc, Words{{q0.x, kWide ? q1.x : 0u, q0.y, kWide ? q1.y : 0u}},
+                                 x.x, x.y);
+                        mma_bf16(acc, Words{{q0.z, kWide ? q1.z : 0u, q0.w, kWide ? q1.w : 0u}},
+                                 x.z, x.w);
                     }
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
@@ -1107,7 +1130,8 @@ attention_join_kernel(const AttentionParams p, int part_rows) {
         const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
         *reinterpret_cast<uint2*>(p.out + i * p.out_stride + (head * p.group + row0 + row) * D +
                                   4 * lane) =
-            make_uint2(pack_bf16x2(r.o.x * inv, r.o.y * inv), pack_bf16x2(r.o.z * inv, r.o.w * inv));
+            make_uint2(pack_bf16x2(r.o.x * inv, r.o.y * inv),
+                       pack_bf16x2(r.o.z * inv, r.o.w * inv));
     };
     if (gridDim.z == 1 && c1 - c0 <= FEW) {
         for (int row = warp; row < rows; row += JOIN_WARPS) store(row, gather(row, c0, 1));
@@ -1210,21 +1234,22 @@ extern "C" int fu_kvcache_append(const fu_kvcache* c, const void* k, const void*
     const int64_t units = cu_seqlens == nullptr ? seqs : kvcache::unit_base(tokens, seqs);
     DeviceGuard guard(c->device);
     if (!guard.ok()) return set_error(FU_ERR_INVALID, "device %d is not available", c->device);
-    Launch launch(dim3(static_cast<unsigned>(units), c->kv_heads, 2), dim3(kvcache::APPEND_THREADS), 0,
-                  stream, (flags & FU_FWD_NO_PDL) == 0);
+    Launch launch(dim3(static_cast<unsigned>(units), c->kv_heads, 2),
+                  dim3(kvcache::APPEND_THREADS), 0, stream, (flags & FU_FWD_NO_PDL) == 0);
     cudaError_t e = cudaLaunchKernelEx(&launch.cfg, kvcache::append_kernel, p);
     if (e != cudaSuccess) return set_error(FU_ERR_CUDA, "launch failed: %s", cudaGetErrorString(e));
     return FU_OK;
 }
 
 typedef void (*SplitKernel)(kvcache::AttentionParams);
-static SplitKernel split_kernel(bool wide, int mode) {
-    static const SplitKernel kernels[2][4] = {
-        {kvcache::attention_split_kernel<false, 0>, kvcache::attention_split_kernel<false, 1>,
-         kvcache::attention_split_kernel<false, 2>, kvcache::attention_split_kernel<false, 3>},
-        {kvcache::attention_split_kernel<true, 0>, kvcache::attention_split_kernel<true, 1>,
-         kvcache::attention_split_kernel<true, 2>, kvcache::attention_split_kernel<true, 3>}};
-    return kernels[wide][mode];
+constexpr int MODES = 6;
+template <bool kWide>
+static SplitKernel split_kernel(int n) {
+    static const SplitKernel kernels[MODES] = {
+        kvcache::attention_split_kernel<kWide, 0>, kvcache::attention_split_kernel<kWide, 2>,
+        kvcache::attention_split_kernel<kWide, 1>, kvcache::attention_split_kernel<kWide, 3>,
+        kvcache::attention_split_kernel<kWide, 5>, kvcache::attention_split_kernel<kWide, 7>};
+    return kernels[n];
 }
 
 // CTAs of the split kernel on a device: two per SM (its shared memory allows no
@@ -1250,8 +1275,9 @@ static int split_ctas(int device) {
 static cudaError_t prepare_split(int device) {
     static std::atomic<bool> done[MAX_DEVICES];
     if (done[device].load(std::memory_order_acquire)) return cudaSuccess;
-    for (int k = 0; k < 8; ++k) {
-        cudaError_t e = cudaFuncSetAttribute(split_kernel(k >> 2, k & 3),
+    for (int k = 0; k < 2 * MODES; ++k) {
+        cudaError_t e = cudaFuncSetAttribute(k < MODES ? split_kernel<false>(k)
+                                                       : split_kernel<true>(k - MODES),
                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              sizeof(kvcache::SplitSmem));
         if (e != cudaSuccess) return e;
@@ -1284,8 +1310,8 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
     if (rc == FU_OK) rc = kvcache::check_rows(out, out_stride, q_heads, "out");
     if (rc == FU_OK) rc = kvcache::check_batch(slots, seq_lens, seqs, status_host);
     if (rc != FU_OK) return rc;
-    if (!(softcap >= 0.f) || !std::isfinite(softcap) || !std::isfinite(scale))
-        return set_error(FU_ERR_INVALID, "scale must be finite, softcap finite and 0 or more");
+    rc = check_scores(scale, softcap);
+    if (rc != FU_OK) return rc;
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
         workspace_bytes < fu_kvcache_attention_workspace(c->device, q_heads, c->kv_heads, seqs))
         return set_error(FU_ERR_INVALID, "workspace too small or not 16-byte aligned");
@@ -1332,7 +1358,9 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
     const bool unsplit = c->max_blocks <= SHORT_BLOCKS && largest <= p.workers / 4;
     p.min_share = unsplit ? 2 * c->max_blocks + 3 : kvcache::MIN_SHARE;
     const bool wide = p.group > 8, pdl = (flags & FU_FWD_NO_PDL) == 0;
-    const int mode = (softcap > 0.f ? 1 : 0) | (alibi_slopes != nullptr ? 2 : 0);
+    const int capped = softcap == 0.f ? 0 : softcap <= kvcache::FINE ? 1 : 2;
+    const int mode = 2 * capped + (alibi_slopes != nullptr);
+    const SplitKernel kernel = wide ? split_kernel<true>(mode) : split_kernel<false>(mode);
     const int smem = sizeof(kvcache::SplitSmem);
     cudaError_t e = prepare_split(c->device);
     if (e != cudaSuccess)
@@ -1344,7 +1372,7 @@ extern "C" int fu_kvcache_attention(const fu_kvcache* c, const void* q, int64_t 
         p.slots = slots + done;
         p.seq_lens = seq_lens + done;
         Launch split(dim3(ctas), dim3(kvcache::SPLIT_THREADS), smem, stream, pdl);
-        e = cudaLaunchKernelEx(&split.cfg, split_kernel(wide, mode), p);
+        e = cudaLaunchKernelEx(&split.cfg, kernel, p);
         if (e == cudaSuccess && !unsplit) {
             const int rows = std::min(p.group, wide ? 16 : 8);
             const bool few = p.seqs * c->kv_heads * p.row_tiles <= p.workers / 4;

@@ -332,6 +332,8 @@ FU_API int fu_oproj_last_grid(const fu_oproj_ctx* ctx);
  *     x_ij  = softcap * tanh(x_ij / softcap)      if softcap > 0
  *     x_ij -= alibi_slopes[h] * |i - j|           if alibi_slopes
  *     out_i = sum_j softmax_j(x_ij) v_j
+ * with |scale| up to 1e30, and a softcap within 1e-3 and 1e6 and no less than
+ * 1e-9 |scale|.
  * Scores, softmax and sums are FP32; the weights are rounded to BF16 for the
  * second product and the output is rounded to BF16.  Rows that are not seen
  * take no part, whatever they hold (infinities and NaN included).  Rows

@@ -420,3 +420,16 @@ def test_decode_deals_every_block_once():
                     assert got[i, pair, 0] == got[i, pair, -(-n // 64) - 1] == c0
                 else:
                     assert all(partial[c, c == c0] == (i, pair) for c in range(c0, c1))
+
+
+@pytest.mark.parametrize("change", [dict(softcap=1e-4), dict(softcap=1e7), dict(scale=1e31),
+                                    dict(scale=2e9, softcap=1.0), dict(scale=float("nan")),
+                                    dict(softcap=float("inf"))])
+def test_scores_that_leave_the_range_are_refused(ctx, change):
+    q, k, v = q_k_v()
+    with pytest.raises(ValueError, match="within"):
+        ctx.ulysses_attention_forward(q, k, v, **change)
+    cache = ctx.create_kv_cache(4, 2, 2)
+    i = torch.zeros(6, dtype=I32)
+    with pytest.raises(ValueError, match="within"):
+        ctx.kv_cache_attention(cache, q, i, i, **change)

@@ -281,3 +281,20 @@ def test_bad_lengths_are_reported(cu):
         check(ctx, q, k, v, 4, 1)
     finally:
         ctx.close()
+
+
+@pytest.mark.parametrize("softcap", [1e-3, 0.1, 1e3, 3e4, 1e6])
+@pytest.mark.parametrize("scale", [None, 1e-4])
+def test_any_cap(contexts, softcap, scale):
+    """Caps far above the scores leave them as they are, to FP32's precision."""
+    check(contexts(4, 1), *make(300, 4, 1, gain=3.0), 4, 1, softcap=softcap, scale=scale)
+
+
+@pytest.mark.parametrize("softcap", [500.0, 1e5])
+def test_one_score_beyond_a_large_cap(contexts, softcap):
+    """A key beyond the cap for half of the rows, in the tile of keys far below it."""
+    q, k, v = make(300, 4, 1, seed=3)
+    k[7] *= 3 * softcap
+    k[140] *= softcap
+    check(contexts(4, 1), q, k, v, 4, 1, softcap=softcap)
+    check(contexts(4, 1), q, k, v, 4, 1, softcap=softcap, causal=False)

@@ -545,3 +545,27 @@ def test_decode_reports_and_skips(slots, lens, match):
         assert_close(out[0], want, size)
     finally:
         ctx.close()
+
+
+@pytest.mark.parametrize("softcap", [1e-3, 0.1, 1e3, 3e4, 1e6])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (12, 1)])
+def test_decode_any_cap(contexts, softcap, q_heads, kv_heads):
+    """Caps far above the scores leave them as they are, to FP32's precision."""
+    ctx = contexts(q_heads, kv_heads)
+    lens = [50, 64, 700]
+    cache, reference, slots = filled(ctx, lens, kv_heads)
+    check_decode(ctx, cache, reference, slots, lens, q_heads, kv_heads, gain=3.0, softcap=softcap)
+
+
+@pytest.mark.parametrize("softcap", [500.0, 1e5])
+def test_decode_one_score_beyond_a_large_cap(contexts, softcap):
+    """A key of the unfinished block beyond the cap for half of the rows."""
+    ctx = contexts(8, 1)
+    gen = generator(21)
+    n = 3 * BLOCK + 40
+    k, v = rows(gen, n, 1), rows(gen, n, 1)
+    k[3 * BLOCK + 5] *= 3 * softcap
+    cache, reference = fresh(ctx, max_seqs=2, max_blocks=4, seed=1), ReferenceCache(1)
+    reference.append(1, k, v)
+    ctx.kv_cache_append(cache, k, v, ints([1]), ints([n]), cu_seqlens=ints([0, n]))
+    check_decode(ctx, cache, reference, [1], [n], 8, 1, softcap=softcap)
