@@ -276,8 +276,10 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
 //     second product needs from it next to 16 bytes of a row of V transposed.
 //   * e4m3 becomes f16 exactly.  (mma.sync with e4m3 operands, q and the weights
 //     as sums of two e4m3, took more instructions per block, 1370 against 1080.)
-//   * q is scaled by a power of two per row, so that f16 holds it; weights are
-//     f16 in [0, 1]; block scales are applied in FP32.
+//   * q is scaled by a power of two per row and the weights by 2^15, so that f16 keeps
+//     11 bits of what is down to 2^-28 (2^-29) of the largest; their sums carry the
+//     same factor.  (Weights in [0, 1] lost bits from 2^-14 on: the many small ones
+//     behind one large score.)  Block scales are applied in FP32.
 // tcgen05 would pad 4 to 16 rows to 128; here the tensor work is far below the
 // time of the loads, and the instructions per block are what has to stay low.
 //
@@ -464,8 +466,8 @@ struct Score {
 };
 
 // One block's scores s[h][j][c] (token 16 t + 2 j + c of the block, already in
-// log2 units, -inf where not seen) -> weights in place, and the factor of what
-// was summed before.
+// log2 units, -inf where not seen) -> weights in place, times 2^15, and the factor of
+// what was summed before.
 template <bool kWide>
 __device__ __forceinline__ void softmax_step(Rows<kWide>& r, float (&s)[Rows<kWide>::H][8][2],
                                              float (&old)[Rows<kWide>::H]) {
@@ -480,11 +482,12 @@ __device__ __forceinline__ void softmax_step(Rows<kWide>& r, float (&s)[Rows<kWi
         old[h] = ex2(r.m[h] - base);
         r.m[h] = top;
         float sum = 0.f;
+        const float from = base - 15.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                s[h][j][c] = ex2(s[h][j][c] - base);
+                s[h][j][c] = ex2(s[h][j][c] - from);
                 sum += s[h][j][c];
             }
         r.l[h] = fmaf(r.l[h], old[h], sum);            // this lane's tokens only
@@ -796,8 +799,8 @@ attention_split_kernel(const AttentionParams p) {
                     top = fmaxf(top, fmaxf(fabsf(bf16_lo(w[k])), fabsf(bf16_hi(w[k]))));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // q = (q 2^-e) 2^e with the row's largest value in [1, 2).
-                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -96), 96);
+                // q = (q 2^-e) 2^e with the row's largest value in [2^14, 2^15).
+                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 141, -96), 96);
                 const float down = __int_as_float((127 - e) << 23);
 #pragma unroll
                 for (int k = 0; k < 16; ++k)

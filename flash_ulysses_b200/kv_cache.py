@@ -77,6 +77,12 @@ class KvCache:
         self._desc = d
         self._address = _C.address_of(d)
 
+    def __setattr__(self, name, value):
+        # Calls read the addresses that the constructor took.
+        if hasattr(self, "_address"):
+            raise AttributeError("a KvCache's tensors are fixed; copy into them instead")
+        super().__setattr__(name, value)
+
     @classmethod
     def allocate(cls, num_blocks, max_seqs, max_blocks, kv_heads, device):
         """A zeroed cache."""

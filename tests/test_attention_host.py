@@ -433,3 +433,11 @@ def test_scores_that_leave_the_range_are_refused(ctx, change):
     i = torch.zeros(6, dtype=I32)
     with pytest.raises(ValueError, match="within"):
         ctx.kv_cache_attention(cache, q, i, i, **change)
+
+
+def test_a_cache_keeps_its_tensors(ctx):
+    cache = ctx.create_kv_cache(4, 2, 2)
+    before = cache.block_table
+    with pytest.raises(AttributeError, match="copy into them"):
+        cache.block_table = torch.zeros(2, 2, dtype=I32)
+    assert cache.block_table is before

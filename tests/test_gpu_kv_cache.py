@@ -569,3 +569,24 @@ def test_decode_one_score_beyond_a_large_cap(contexts, softcap):
     reference.append(1, k, v)
     ctx.kv_cache_append(cache, k, v, ints([1]), ints([n]), cu_seqlens=ints([0, n]))
     check_decode(ctx, cache, reference, [1], [n], 8, 1, softcap=softcap)
+
+
+@pytest.mark.parametrize("lead", [12.0, 17.0, 19.5])
+@pytest.mark.parametrize("q_heads", [4, 12])
+def test_decode_many_small_weights(contexts, lead, q_heads):
+    """One key ahead of all others by `lead`, whose values alone make the output: weights of
+    e^-lead keep their precision."""
+    ctx = contexts(q_heads, 1)
+    n = 10 * BLOCK + 30
+    q = torch.zeros(1, q_heads, DIM, device="cuda")
+    q[..., 0] = DIM ** 0.5
+    q[..., 1] = 2.0 ** -17                               # small next to the row's largest
+    k = torch.zeros(n, DIM, device="cuda")
+    k[5, 0] = lead
+    v = torch.ones(n, DIM, device="cuda")
+    v[5] = 0
+    q, k, v = q.view(1, -1).bfloat16(), k.bfloat16(), v.bfloat16()
+    cache, reference = fresh(ctx, max_seqs=1, max_blocks=11, seed=1), ReferenceCache(1)
+    reference.append(0, k, v)
+    ctx.kv_cache_append(cache, k, v, ints([0]), ints([n]), cu_seqlens=ints([0, n]))
+    check_decode(ctx, cache, reference, [0], [n], q_heads, 1, q=q)
