@@ -298,3 +298,35 @@ def test_one_score_beyond_a_large_cap(contexts, softcap):
     k[140] *= softcap
     check(contexts(4, 1), q, k, v, 4, 1, softcap=softcap)
     check(contexts(4, 1), q, k, v, 4, 1, softcap=softcap, causal=False)
+
+
+@pytest.mark.parametrize("factor", [1e-4, 0.3, 1.0, 1.45, 30.0, -0.7])
+@pytest.mark.parametrize("mode", ["causal", "prefix", "full", "documents"])
+def test_any_slope(contexts, factor, mode):
+    """Slopes from none to ones that leave a row only itself, and a negative one."""
+    options = dict(causal=mode != "full", cu=None)
+    if mode == "documents":
+        options["cu"] = [0, 90, 350, 351, 700]
+    if mode == "prefix":
+        options.update(cu=[0, 300, 700], prefix=[280, 150])
+    slopes = factor * torch.tensor([1.0, 0.5, 0.03, 0.002], device="cuda")
+    check(contexts(4, 1), *make(700, 4, 1, seed=11, gain=3.0), 4, 1, slopes=slopes, **options)
+    check(contexts(4, 1), *make(700, 4, 1, seed=12, gain=3.0), 4, 1, slopes=slopes, softcap=8.0,
+          **options)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-30, -0.1])
+def test_slopes_with_any_scale(contexts, scale):
+    q, k, v = make(500, 4, 1, seed=13)
+    for size in (1.0, 1e-20, 1e20):
+        check(contexts(4, 1), q, k, (v.float() * size).bfloat16(), 4, 1, slopes=slopes_of(4),
+              scale=scale, cu=[0, 3, 260, 500])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_documents_that_share_a_warp(contexts, causal):
+    """Boundaries at every place of a warp's 32 rows, long documents next to short ones."""
+    cu = [0, 1, 33, 66, 100, 135, 171, 460, 463, 900, 901, 1000]
+    for slopes in (None, slopes_of(4)):
+        check(contexts(4, 1), *make(1024, 4, 1, seed=14, gain=2.0), 4, 1, cu=cu, causal=causal,
+              slopes=slopes)

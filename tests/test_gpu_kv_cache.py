@@ -590,3 +590,12 @@ def test_decode_many_small_weights(contexts, lead, q_heads):
     reference.append(0, k, v)
     ctx.kv_cache_append(cache, k, v, ints([0]), ints([n]), cu_seqlens=ints([0, n]))
     check_decode(ctx, cache, reference, [0], [n], q_heads, 1, q=q)
+
+
+def test_decode_more_sequences_than_a_launch_takes(contexts):
+    """Sequences go 1024 to a launch; the launches share their scratch."""
+    ctx = contexts(2, 1)
+    lens = [1 + (53 * i) % 90 for i in range(1500)]
+    lens[1100] = 5000
+    cache, reference, slots = filled(ctx, lens, 1)
+    check_decode(ctx, cache, reference, slots, lens, 2, 1)
