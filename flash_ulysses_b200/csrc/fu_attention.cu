@@ -717,7 +717,7 @@ __device__ void run_softmax(const Params& p, uint8_t* smem, uint32_t tmem, const
         const bool valid = seen.x < seen.y;
         // A row without a document is computed like one that sees everything, and not
         // stored.
-        const int lo = valid ? seen.x : INT_MIN / 2, hi = valid ? seen.y : INT_MAX / 2;
+        const int lo = valid ? seen.x : 0, hi = valid ? seen.y : INT_MAX / 2;
         // What some and what all of the warp's rows of documents see.
         constexpr uint32_t ALL = 0xffffffffu;
         const int lo_some = __reduce_min_sync(ALL, valid ? seen.x : INT_MAX);
