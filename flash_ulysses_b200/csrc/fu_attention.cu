@@ -1,9 +1,9 @@
 // Attention over the exchanged Q/K/V rows (sm_100a): packed documents, causal,
 // prefix or full masks, scores capped by a tanh and/or lowered with distance.
 //
-// A CTA takes items -- one query head's 256 rows, as two tiles of 128 -- and for
-// each walks the keys that any of the rows sees in tiles of 128 with an online
-// softmax:
+// A CTA takes items -- one query head's 256 rows, as two tiles of 128, or 128 rows
+// where there are few -- and for each walks the keys that any of the rows sees in
+// tiles of 128 with an online softmax:
 //     S = Q K^T          tcgen05, Q and K from shared memory, S in TMEM
 //     m' = max(m, S), P = 2^(c S - c m'), l = l 2^(c m - c m') + sum P
 //     O = O 2^(c m - c m') + P V     tcgen05, P from TMEM, V from shared memory
@@ -55,12 +55,13 @@ namespace attention {
 
 constexpr int D = FU_HEAD_DIM;
 constexpr int TILE = 128;                       // rows of a query tile, keys of a key tile
-constexpr int ROWS = 2 * TILE;                  // query rows per CTA
+constexpr int ROWS = 2 * TILE;                  // query rows of an item, or (few items) TILE
 constexpr int NUM_THREADS = 384;
 constexpr int TILE_BYTES = TILE * D * 2;        // 32 KiB: two 64-column boxes
 constexpr int BOX_BYTES = TILE_BYTES / 2;
 constexpr int STAGES = 5;                       // K and V tiles in turn
 constexpr int SLOTS = 4;                        // items handed out and not finished
+constexpr int SMS = 148;
 constexpr int MAX_RANKED = 256;                 // row blocks that are put in order of their length
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = OFF_Q + 2 * TILE_BYTES;
@@ -102,6 +103,7 @@ struct Params {
     int32_t tokens, docs, q_heads, group, causal;
     int32_t key_step;                  // from a key tile to the next: 128, or -128 (below)
     int32_t row_blocks;                // row_blocks * q_heads items, a CTA of the grid each
+    int32_t block_rows;                // rows of an item: 256 or 128
     int32_t ranked;                    // row blocks go by length, else from the last to the first
     int32_t wide_store;                // out rows are 32-byte aligned
     uint32_t negate;                   // scale < 0: the MMA negates Q, `scale` is positive
@@ -443,8 +445,8 @@ __device__ void run_loads(const Params& p, uint8_t* smem, const Bars& b, volatil
         if (k >= 0) {
             const int block = k / p.q_heads;
             const int head = k - block * p.q_heads;
-            const int row0 = (p.ranked ? rank[block] : p.row_blocks - 1 - block) * ROWS;
-            const int valid = min(rows - row0, ROWS);
+            const int row0 = (p.ranked ? rank[block] : p.row_blocks - 1 - block) * p.block_rows;
+            const int valid = min(rows - row0, p.block_rows);
             if (valid > 0) w = make_item(p, row0, head, valid);
             if (w.tiles <= 0) {        // (0: cu_seqlens that make no sense)
                 k = claim();
@@ -1034,11 +1036,11 @@ attention_kernel(const __grid_constant__ Params p) {
         const int me = threadIdx.x, rows = document_rows(p);
         int mine = 0;
         if (me < p.row_blocks) {
-            const int valid = min(rows - me * ROWS, ROWS);
+            const int row0 = me * p.block_rows, valid = min(rows - row0, p.block_rows);
             int kv0 = 0;
             for (int t = 0; t < 2 && valid > t * TILE; ++t) {
-                const int2 head = seen_rows(p, me * ROWS + t * TILE);
-                const int2 tail = seen_rows(p, me * ROWS + min(valid, (t + 1) * TILE) - 1);
+                const int2 head = seen_rows(p, row0 + t * TILE);
+                const int2 tail = seen_rows(p, row0 + min(valid, (t + 1) * TILE) - 1);
                 if (t == 0) kv0 = head.x;
                 int first, last;
                 tile_range(head, tail, kv0, first, last);
@@ -1152,7 +1154,14 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
         return set_error(FU_ERR_DEVICE, "an earlier launch reported device status 0x%x",
                          static_cast<unsigned>(*a->status_host));
 
-    const int64_t blocks = (a->tokens + attention::ROWS - 1) / attention::ROWS * a->q_heads;
+    // Two tiles of 128 rows keep a CTA's tensor cores busy in turn.  Where the call has at
+    // most two tiles per SM an item is one tile: more CTAs, and shorter ones.  (700 tokens of
+    // 8 heads 14.1 us, 15.9 us with two; 2048 of 4 heads 30.3 and 32.2 us; 6800 of 4 heads, 216
+    // tiles, 88.8 and 92.5 us.)
+    const int64_t tiles = (a->tokens + attention::TILE - 1) / attention::TILE;
+    const int block_rows = tiles * a->q_heads <= 2 * attention::SMS ? attention::TILE : attention::ROWS;
+    const int64_t row_blocks = (a->tokens + block_rows - 1) / block_rows;
+    const int64_t blocks = row_blocks * a->q_heads;
     if (blocks > INT32_MAX)
         return set_error(FU_ERR_INVALID, "tokens * q_heads is too large for one call");
 
@@ -1180,7 +1189,8 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
     p.q_heads = a->q_heads;
     p.group = a->q_heads / a->kv_heads;
     p.causal = a->causal;
-    p.row_blocks = static_cast<int32_t>((a->tokens + attention::ROWS - 1) / attention::ROWS);
+    p.row_blocks = static_cast<int32_t>(row_blocks);
+    p.block_rows = block_rows;
     p.ranked = a->cu_seqlens != nullptr && p.row_blocks > 1 && p.row_blocks <= attention::MAX_RANKED;
     p.wide_store = (reinterpret_cast<uintptr_t>(a->out) | a->out_stride * 2) % 32 == 0;
     p.negate = a->scale < 0.f ? 1u : 0u;

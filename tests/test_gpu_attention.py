@@ -330,3 +330,38 @@ def test_documents_that_share_a_warp(contexts, causal):
     for slopes in (None, slopes_of(4)):
         check(contexts(4, 1), *make(1024, 4, 1, seed=14, gain=2.0), 4, 1, cu=cu, causal=causal,
               slopes=slopes)
+
+
+@pytest.mark.parametrize("softcap,alibi,prefix,causal", [
+    (0.0, False, False, True), (0.0, False, False, False), (30.0, True, True, True),
+    (5.0, False, True, True), (0.0, True, False, False), (0.0, True, True, True),
+])
+@pytest.mark.parametrize("cu,n", [(None, 700), ((0, 1, 1, 130, 131, 400, 700), 700),
+                                  ((0, 256, 512, 640), 700), ((0, 300, 310, 600), 641)])
+def test_two_tiles_an_item(contexts, softcap, alibi, prefix, causal, cu, n):
+    """64 heads: enough tiles of 128 rows for two of them to share an item."""
+    lens = None if not prefix else [(37 * (d + 3)) % 200 for d in range(len(cu or (0, 1)) - 1)]
+    check(contexts(64, 2), *make(n, 64, 2, seed=15, gain=2.0), 64, 2, cu=cu, prefix=lens,
+          causal=causal, softcap=softcap, slopes=slopes_of(64) if alibi else None)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_two_tiles_an_item_and_what_is_not_seen(contexts, bad):
+    """Values that rows do not see hold infinities or NaN, in K and in V."""
+    q, k, v = make(700, 64, 2, seed=16)
+    clean = v.clone()
+    v[100:130] = bad
+    k[100:130] = bad
+    cu = [0, 100, 130, 385, 650]
+    ctx = contexts(64, 2)
+    got = ctx.ulysses_attention_forward(q, k, v, cu_seqlens=ints(cu))
+    ctx.check()
+    want, size = attention(q, torch.nan_to_num(k.float()).bfloat16(), clean, 64, 2, cu)
+    for a, b in ((0, 100), (130, 650)):
+        assert_close(got[a:b], want[a:b], size[a:b])
+
+
+@pytest.mark.parametrize("n", [1, 127, 128, 129, 255, 256, 257, 500, 513])
+def test_two_tiles_an_item_lengths(contexts, n):
+    heads = 296 // ((n + 127) // 128) + 1
+    check(contexts(heads, 1), *make(n, heads, 1, seed=n), heads, 1)
