@@ -623,24 +623,39 @@ __device__ void run_mma(const Params& p, uint8_t* smem, uint32_t tmem, const Bar
 }
 
 // ------------------------------------------------------------ V at a mask's edge
-// Every V tile is counted (on a ring of barriers of its own), so that neither
-// side gets more than the ring ahead; only those at an edge are looked at.
+// These warps take every load off the ring in its order, K tiles too, and give each
+// stage back as the products do: by its parity alone a phase of kv_full cannot be told
+// from the one two before or behind, so a warp that waits for a stage must have seen its
+// last load, and the stage must not be filled again before it has seen this one.  Every V
+// tile is counted on a ring of barriers of its own; only those at an edge are looked at.
 __device__ void run_clean(const Params& p, uint8_t* smem, const Bars& b,
                           volatile int* abort_flag) {
     const int me = threadIdx.x & 63;
-    int stage = 1, count = 0;          // of the next V tile: ring stage, place on its own ring
+    int stage = 0, count = 0;          // ring stage of the next load, place of the next V tile
     uint32_t use = 0;
+    const auto full = [&]() {
+        return __all_sync(0xffffffffu, fu_wait_parity(b.kv_full + 8 * stage, use, abort_flag,
+                                                      p.timeout_ns, p.status, W_KV_FULL));
+    };
+    const auto give_back = [&]() {
+        __syncwarp();
+        if ((me & 31) == 0) mbar_arrive(b.kv_empty + 8 * stage);
+        if (++stage == STAGES) {
+            stage = 0;
+            use ^= 1;
+        }
+    };
     for (int n = 0;; ++n) {
         const int slot = n % SLOTS;
-        bool ok = fu_wait_parity(b.item_full + 8 * slot, (n / SLOTS) & 1, abort_flag, p.timeout_ns,
-                                 p.status, W_ITEM);
+        const bool ok = fu_wait_parity(b.item_full + 8 * slot, (n / SLOTS) & 1, abort_flag,
+                                       p.timeout_ns, p.status, W_ITEM);
         if (!__all_sync(0xffffffffu, ok)) return;
         Item& w = *reinterpret_cast<Item*>(smem + OFF_ITEM + 64 * slot);
         const int tiles = w.tiles;
         for (int j = 0; j < tiles; ++j) {
-            ok = fu_wait_parity(b.kv_full + 8 * stage, use, abort_flag, p.timeout_ns, p.status,
-                                W_KV_FULL);
-            if (!__all_sync(0xffffffffu, ok)) return;
+            if (!full()) return;                       // K
+            give_back();
+            if (!full()) return;                       // V
             if (w.edge(j)) {
                 uint4* v = reinterpret_cast<uint4*>(smem + OFF_KV + stage * TILE_BYTES);
                 // A BF16 is not finite if its exponent bits are all set; one more then
@@ -669,11 +684,7 @@ __device__ void run_clean(const Params& p, uint8_t* smem, const Bars& b,
             __syncwarp();
             if ((me & 31) == 0) mbar_arrive(b.clean + 8 * count);
             if (++count == STAGES) count = 0;
-            stage += 2;
-            if (stage >= STAGES) {
-                stage -= STAGES;
-                use ^= 1;
-            }
+            give_back();
         }
         __syncwarp();
         if ((me & 31) == 0) mbar_arrive(b.item_empty + 8 * slot);
@@ -990,7 +1001,7 @@ attention_kernel(const __grid_constant__ Params p) {
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(b.kv_full + 8 * s, 1);
-            mbar_init(b.kv_empty + 8 * s, 1);
+            mbar_init(b.kv_empty + 8 * s, 3);          // the products, two cleaning warps
             mbar_init(b.clean + 8 * s, 2);
         }
         for (int t = 0; t < 2; ++t) {
