@@ -485,7 +485,9 @@ class FlashUlyssesContext:
         the rest stays in the slot's tail.  A slot may occur only once in a
         call.  Slots, blocks or lengths that do not fit the cache are reported
         like every device-side error, by the next call or ``check()``, and
-        nothing is written for them.
+        nothing is written for them.  Where it was a block, the sequence's
+        earlier tokens are kept, and the call may be made again for it with
+        the table put right.
         """
         _check_cache(cache, self._widths[1], self.device)
         if _C.try_append is not None and self._widths[2] >= 0:

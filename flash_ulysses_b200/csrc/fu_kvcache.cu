@@ -74,10 +74,12 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d
 // for K, dims x tokens for V) are words of four bytes.  Each new row is read once
 // and leaves as half its bytes; what bounds it is the chain of its loads (the
 // sequence, its length, the rows) in two rounds of CTAs: 8192 rows of 8 heads take
-// 13.0 us, 4.0 TB/s, where memory alone would take 7.9 us.  One trip to memory is
-// all that the search and the check for slots named twice add to that chain.
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendParams p) {
-    __shared__ uint32_t s_max[4];
+// 13.2 us, 3.9 TB/s, where memory alone would take 7.9 us.  One trip to memory is
+// all that the search and the check for slots named twice add to that chain.  Unbounded
+// the kernel would take 63 registers and 8 CTAs fit on an SM: 13.4 us; with 9, 13.2 us.
+__global__ void __launch_bounds__(APPEND_THREADS, 9) append_kernel(const AppendParams p) {
+    constexpr uint32_t KEEP_TAIL = 1u << 31;
+    __shared__ uint32_t s_max[4];                      // of a warp, and KEEP_TAIL
     __shared__ uint32_t s_v[D * PITCH];
     grid_dependency_wait();
     grid_launch_dependents();
@@ -133,13 +135,15 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
     __nv_bfloat16* tail = p.tail[which] + (static_cast<int64_t>(slot) * p.kv_heads + h) * BLOCK * D;
     const int tg = t >> 4, c = t & 15;                 // token group (and tg + 8), 8-dim chunk
 
+    bool keep_tail = false;
     if (b >= full) {
         if (__syncthreads_or(again)) {
             if (threadIdx.x == 0) report_status(p.status, FU_DEV_SLOT_TWICE, W_APPEND);
             return;
         }
     } else {
-        const int id = __ldg(p.block_table + static_cast<int64_t>(slot) * p.max_blocks + b);
+        const int32_t* table = p.block_table + static_cast<int64_t>(slot) * p.max_blocks;
+        const int id = __ldg(table + b);
         // Tokens of this block held before the call are in the tail.
         uint4 x[2][4];
 #pragma unroll
@@ -166,12 +170,23 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
             for (int k = 0; k < 32; ++k) best = finite_max(words[k], best);
         }
         best = __reduce_max_sync(0xffffffffu, best);
+        // A tail that holds tokens of a block that is done now is their only source when a
+        // call that met a block outside the cache is made again: then it stays.
+        if (j == 0 && start % BLOCK != 0) {
+            bool outside = false;
+            for (int o = b + t; o < full; o += APPEND_THREADS)
+                outside |= static_cast<uint32_t>(__ldg(table + o)) >=
+                           static_cast<uint32_t>(p.num_blocks);
+            if (__any_sync(0xffffffffu, outside)) best |= KEEP_TAIL;
+        }
         if (lane == 0) s_max[t >> 5] = best;
         if (__syncthreads_or(again)) {
             if (threadIdx.x == 0) report_status(p.status, FU_DEV_SLOT_TWICE, W_APPEND);
             return;
         }
-        best = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
+        keep_tail = ((s_max[0] | s_max[1] | s_max[2] | s_max[3]) & KEEP_TAIL) != 0;
+        best = max(max(s_max[0] & ~KEEP_TAIL, s_max[1] & ~KEEP_TAIL),
+                   max(s_max[2] & ~KEEP_TAIL, s_max[3] & ~KEEP_TAIL));
         // best = (1 + m / 128) 2^(e - 127) in BF16's bits; 448 = 1.75 * 2^8.
         const int e = best >> 7;
         const int power = max(e - 127 - 8 + ((best & 127u) > 96u ? 1 : 0), -126);
@@ -236,7 +251,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const AppendPara
     }
     // The first unit, which alone reads the tail, also writes the rows of the
     // block that stays unfinished (after the barriers above when it read it).
-    if (j == 0) {
+    if (j == 0 && !keep_tail) {
         const int first = max(full * BLOCK - start, 0);     // first row that goes to the tail
         for (int o = t; o < (n - first) * 16; o += 128) {   // (fewer than 64 rows)
             const int r = first + (o >> 4), at = (start + r) % BLOCK;

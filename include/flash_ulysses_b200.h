@@ -411,10 +411,13 @@ typedef struct fu_kvcache {
  * sequence i are [cu_seqlens[i], cu_seqlens[i + 1]) (seqs + 1 device words,
  * from 0, not decreasing, up to tokens).  slots and seq_lens are device
  * int32 [seqs].  A negative slot is skipped (a padded batch).  Skipped and
- * reported: a slot that an earlier row names too (FU_STATUS_SLOT_TWICE), a
- * slot or block outside the cache (FU_STATUS_CACHE_RANGE), a length below n_i
- * or above max_blocks * 64, or rows that cu_seqlens puts outside the call
- * (FU_STATUS_LENGTHS). */
+ * reported: a slot that an earlier sequence of the call names too, if only for
+ * no rows (FU_STATUS_SLOT_TWICE), a slot or block outside the cache
+ * (FU_STATUS_CACHE_RANGE), a length below n_i or above max_blocks * 64, or rows
+ * that cu_seqlens puts outside the call (FU_STATUS_LENGTHS).  Of a sequence with
+ * a block outside the cache the other blocks are written, and the tail unless
+ * it holds earlier tokens: the same call may be made again for that sequence,
+ * with the table put right, and leaves what it would have left at once. */
 FU_API int fu_kvcache_append(const fu_kvcache* cache, const void* k, const void* v,
                              int64_t k_stride, int64_t v_stride, int64_t tokens,
                              const int32_t* slots, const int32_t* seq_lens,
