@@ -478,7 +478,9 @@ class FlashUlyssesContext:
         included.  With ``cu_seqlens`` (int32, ``[n + 1]``, from 0, not
         decreasing) rows ``cu_seqlens[i]`` up to ``cu_seqlens[i + 1]`` are the
         next tokens of slot ``slots[i]``, whose length becomes ``seq_lens[i]``
-        (both ``[n]``); rows behind its last entry are not read.
+        (both ``[n]``); rows behind its last entry are not read.  One that
+        decreases is reported, and sequences of the call may then be written
+        in part.
 
         A negative slot is skipped, so a batch may be padded.  Blocks that the
         call completes are written to ``cache.block_table``'s blocks in 8 bits;

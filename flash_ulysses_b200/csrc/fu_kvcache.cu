@@ -74,9 +74,9 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d
 // for K, dims x tokens for V) are words of four bytes.  Each new row is read once
 // and leaves as half its bytes; what bounds it is the chain of its loads (the
 // sequence, its length, the rows) in two rounds of CTAs: 8192 rows of 8 heads take
-// 13.2 us, 3.9 TB/s, where memory alone would take 7.9 us.  One trip to memory is
+// 13.4 us, 3.9 TB/s, where memory alone would take 7.9 us.  One trip to memory is
 // all that the search and the check for slots named twice add to that chain.  Unbounded
-// the kernel would take 63 registers and 8 CTAs fit on an SM: 13.4 us; with 9, 13.2 us.
+// the kernel would take 63 registers and 8 CTAs fit on an SM: 13.6 us; with 9, 13.4 us.
 __global__ void __launch_bounds__(APPEND_THREADS, 9) append_kernel(const AppendParams p) {
     constexpr uint32_t KEEP_TAIL = 1u << 31;
     __shared__ uint32_t s_max[4];                      // of a warp, and KEEP_TAIL
@@ -89,6 +89,14 @@ __global__ void __launch_bounds__(APPEND_THREADS, 9) append_kernel(const AppendP
     const int t = threadIdx.x, lane = threadIdx.x & 31;
     int i = blockIdx.x, j = 0, row0 = i, n = 1;
     if (p.cu_seqlens != nullptr) {
+        // All of cu_seqlens is looked at once, by the last unit, which never has rows of its
+        // own: where an entry decreases, the search may pass by the sequence that shows it.
+        if (blockIdx.x == gridDim.x - 1 && h == 0 && which == 0)
+            for (int d = t; d < p.seqs; d += APPEND_THREADS) {
+                const int c0 = __ldg(p.cu_seqlens + d), c1 = __ldg(p.cu_seqlens + d + 1);
+                if (c1 < c0 || c1 > p.tokens || (d == 0 && c0 != 0))
+                    report_status(p.status, FU_DEV_LENGTHS, W_APPEND);
+            }
         // The last sequence whose units begin at this one or before: a 32-ary search,
         // one trip to memory up to 32 sequences.
         int lo = 0, count = p.seqs;

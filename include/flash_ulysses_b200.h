@@ -414,7 +414,9 @@ typedef struct fu_kvcache {
  * reported: a slot that an earlier sequence of the call names too, if only for
  * no rows (FU_STATUS_SLOT_TWICE), a slot or block outside the cache
  * (FU_STATUS_CACHE_RANGE), a length below n_i or above max_blocks * 64, or rows
- * that cu_seqlens puts outside the call (FU_STATUS_LENGTHS).  Of a sequence with
+ * that cu_seqlens puts outside the call (FU_STATUS_LENGTHS).  Where cu_seqlens
+ * decreases, which is reported too, other sequences of the call may be written
+ * in part.  Of a sequence with
  * a block outside the cache the other blocks are written, and the tail unless
  * it holds earlier tokens: the same call may be made again for that sequence,
  * with the table put right, and leaves what it would have left at once. */

@@ -85,3 +85,40 @@ def test_a_token_that_completes_a_block_outside_the_cache(ctx):
     for slot in (0, 1):
         reference.append(slot, k[slot:slot + 1], v[slot:slot + 1])
     assert_holds(cache, reference, [0, 1])
+
+
+@pytest.mark.parametrize("cu,tokens", [([0, 1000, 0, 0], 1000), ([0, 200, 100, 150], 200),
+                                       ([0, 10, 5, 10, 15, 20], 20), ([3, 10, 20], 20),
+                                       ([0, 5, 21], 20), ([0, -1, 5], 20)])
+def test_every_entry_of_cu_seqlens_is_checked(ctx, cu, tokens):
+    """Also one that the search for a work unit's sequence passes by.  Slots that the call does not
+    name, and blocks that are not theirs, stay as they were."""
+    cache = fresh(ctx, max_seqs=8, max_blocks=20)
+    count = len(cu) - 1
+    before = state_of(cache)
+    k, v = rows(generator(1), tokens, 2), rows(generator(2), tokens, 2)
+    ctx.kv_cache_append(cache, k, v, ints(range(count)), ints([1000] * count),
+                        cu_seqlens=ints(cu))
+    with pytest.raises(RuntimeError, match="cu_seqlens"):
+        ctx.check()
+    ctx.clear_error()
+    mine = cache.block_table[:count].flatten().tolist()
+    others = [b for b in range(cache.num_blocks) if b not in mine]
+    for t, old in zip(state_of(cache)[:4], before[:4]):
+        assert torch.equal(t[others], old[others])
+    for t, old in zip(state_of(cache)[4:], before[4:]):
+        assert torch.equal(t[count:], old[count:])
+
+
+def test_one_bad_entry_among_many(ctx):
+    count = 1000
+    cache = fresh(ctx, max_seqs=count, max_blocks=1)
+    k, v = rows(generator(1), count, 2), rows(generator(2), count, 2)
+    for at in (1, 333, 998):
+        cu = list(range(count + 1))
+        cu[at], cu[at + 1] = cu[at + 1], cu[at]
+        ctx.kv_cache_append(cache, k, v, ints(range(count)), ints([2] * count),
+                            cu_seqlens=ints(cu))
+        with pytest.raises(RuntimeError, match="cu_seqlens"):
+            ctx.check()
+        ctx.clear_error()
