@@ -406,6 +406,17 @@ __device__ __forceinline__ int claimed_cta(uint32_t answer) {
     return got ? static_cast<int>(x) : -1;
 }
 
+// Reports document ends that do not start at 0, decrease or leave the call, by a whole warp.
+__device__ void check_cu_seqlens(const Params& p) {
+    for (int d = threadIdx.x & 31; d <= p.docs; d += 32) {
+        const int x = __ldg(p.cu_seqlens + d);
+        const int before = d > 0 ? __ldg(p.cu_seqlens + d - 1) : 0;
+        if (x < before || x > p.tokens || (d == 0 && x != 0))
+            report_status(p.status, FU_DEV_LENGTHS, W_CU_SEQLENS);
+    }
+    __syncwarp();
+}
+
 // Ring order per item: K_0, V_0, K_1, V_1, ...  The whole warp works out the
 // items, its first lane loads.
 __device__ void run_loads(const Params& p, uint8_t* smem, const Bars& b, volatile int* abort_flag) {
@@ -428,6 +439,9 @@ __device__ void run_loads(const Params& p, uint8_t* smem, const Bars& b, volatil
     // for when this one's last loads are out.
     const uint32_t answer = smem_u32(smem + OFF_MISC + 16);
     const auto claim = [&]() {
+        // Once a call, with the first item: its CTA may have been taken over like any
+        // other.  Its loads are out, so nothing waits for this.
+        if (k == 0 && p.cu_seqlens != nullptr) check_cu_seqlens(p);
         if (lane == 0) {
             mbar_arrive_expect_tx(b.next, 16);
             claim_cta(answer, b.next);
@@ -1032,14 +1046,6 @@ attention_kernel(const __grid_constant__ Params p) {
     grid_dependency_wait();
     grid_launch_dependents();
 
-    if (blockIdx.x == 0 && p.cu_seqlens != nullptr) {
-        for (int d = threadIdx.x; d <= p.docs; d += NUM_THREADS) {
-            const int x = __ldg(p.cu_seqlens + d);
-            const int before = d > 0 ? __ldg(p.cu_seqlens + d - 1) : 0;
-            if (x < before || x > p.tokens || (d == 0 && x != 0))
-                report_status(p.status, FU_DEV_LENGTHS, W_CU_SEQLENS);
-        }
-    }
     if (p.ranked) {
         // Row blocks by the key tiles that their two query tiles walk, longest
         // first: each counts those that go before it.
