@@ -457,11 +457,11 @@ struct Rows {
 // A score's path from the product to log2 units, and what it needs of a row.  kMode: 1
 // capped by a tanh, 2 lowered with distance, 4 (with 1) by a cap above FINE.
 //
-// With x = 2 log2(e) z, cap tanh(z) = cap (1 - 2 / (1 + 2^x)) is off by 2^-22 cap: up to
-// a cap of FINE a small part of what rounding the weights to f16 costs.  Larger caps
-// matter for scores far below them, which take an odd polynomial of degree 7 in z, off
-// by 2e-7 with the slope at 0 exact: relative to the score it is off by 2^-21 whatever
-// the cap.  (Both forms in one kernel: 34.8 us instead of 33.5 us for 256 sequences of up to
+// With x = 2 log2(e) z, cap tanh(z) = cap (1 - 2 / (1 + 2^x)) is off by less than 2^-21
+// cap: up to a cap of FINE a small part of what rounding the weights to f16 costs.  Larger
+// caps matter for scores far below them, which take an odd polynomial of degree 7 in z, off
+// by 2e-7 with the slope at 0 exact: relative to the score it is off by less than 2^-19
+// (1.0e-6 and the roundings) whatever the cap.  (Both forms in one kernel: 34.8 us instead of 33.5 us for 256 sequences of up to
 // 1500 tokens with the first.)
 constexpr float FINE = 256.f;
 template <int kMode>
