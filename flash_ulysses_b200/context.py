@@ -32,7 +32,6 @@ projection.
 from __future__ import annotations
 
 import functools
-import math
 
 import torch
 import torch.distributed as dist
@@ -400,7 +399,8 @@ class FlashUlyssesContext:
         into the rows: document ``d`` is rows ``cu_seqlens[d]`` up to
         ``cu_seqlens[d + 1]``, and a row sees rows of its own document only.
         It starts at 0 and does not decrease; rows behind its last entry are
-        not written and have no part in others.  Without it all rows are one
+        not written (undefined if the call makes ``out``) and have no part in
+        others.  Without it all rows are one
         document.
         ``causal=True`` lets a row see itself and the rows before it, and with
         ``prefix_lens`` (int32, ``[documents]``, needs ``causal``) also the
@@ -526,8 +526,8 @@ class FlashUlyssesContext:
         first ``seq_lens[i]`` tokens (int32 ``[n]`` each), so append it first.
         Scores as in ``ulysses_attention_forward``.  Returns BF16
         ``[n, output_q_heads * 128]``, written into ``out`` when given.  A row
-        with a negative slot is left as it was, one with length 0 is zeroed; a
-        slot may occur more than once.  Slots, blocks and lengths that do not
+        with a negative slot is left as it was (undefined if the call makes
+        ``out``), one with length 0 is zeroed; a slot may occur more than once.  Slots, blocks and lengths that do not
         fit the cache are reported by the next call or ``check()``.
         """
         _check_cache(cache, self._widths[1], self.device)

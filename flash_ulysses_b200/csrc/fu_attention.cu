@@ -1218,7 +1218,7 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
     // A bias falls with distance.  From the keys before a row towards it the maximum would
     // grow in every tile, and O be rescaled; from the last key on it is found at once.
     // (8192 causal tokens of 8 heads: 154 us the one way and 134 us the other, before the
-    // bias moved into the exponent, which needs this order; 120 us with both.)
+    // bias moved into the exponent; 120 us with that.)
     p.key_step = a->alibi_slopes != nullptr ? -attention::TILE : attention::TILE;
 
     DeviceGuard guard(a->device);
