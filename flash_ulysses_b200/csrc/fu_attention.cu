@@ -788,8 +788,8 @@ __device__ void run_softmax(const Params& p, uint8_t* smem, uint32_t tmem, const
                 // scores far below it: there the last form takes the polynomial for |z| <= 1,
                 // and a score is off by less than 2^-19 of itself (1.2e-6 and the roundings).
                 // What a cap costs is its instructions between a row's scores and its weights:
-                // 8192 tokens of 8 heads take 1040 a warp and key tile, 680 without, and 160 us
-                // for 113, while no pipe is busy for more than 42 % of the time; the last form
+                // 8192 tokens of 8 heads take 1040 a warp and key tile, 695 without, and 161 us
+                // for 115, while no pipe is busy for more than 46 % of the time; the last form
                 // also takes three special-function results per score with the weight's.
                 constexpr float FINE = 1024.f;
                 const f32x2 to_cap2 = pair(to_cap), lin2 = pair(lin);
@@ -1218,7 +1218,7 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
     // A bias falls with distance.  From the keys before a row towards it the maximum would
     // grow in every tile, and O be rescaled; from the last key on it is found at once.
     // (8192 causal tokens of 8 heads: 154 us the one way and 134 us the other, before the
-    // bias moved into the exponent; 120 us with that.)
+    // bias moved into the exponent; 123 us with that.)
     p.key_step = a->alibi_slopes != nullptr ? -attention::TILE : attention::TILE;
 
     DeviceGuard guard(a->device);

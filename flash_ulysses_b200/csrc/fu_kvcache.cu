@@ -72,11 +72,13 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d
 // holds two groups of 4 tokens x 8 dims: coalesced 16-byte loads, the block's
 // largest value by a reduction over the CTA, and both output orders (tokens x dims
 // for K, dims x tokens for V) are words of four bytes.  Each new row is read once
-// and leaves as half its bytes; what bounds it is the chain of its loads (the
-// sequence, its length, the rows) in two rounds of CTAs: 8192 rows of 8 heads take
-// 13.4 us, 3.9 TB/s, where memory alone would take 7.9 us.  One trip to memory is
-// all that the search and the check for slots named twice add to that chain.  Unbounded
-// the kernel would take 63 registers and 8 CTAs fit on an SM: 13.6 us; with 9, 13.4 us.
+// and leaves as half its bytes.  What bounds it is latency: a CTA is one chain of
+// loads (the sequence, its length, the rows), and there are two rounds of CTAs with
+// nothing in flight between them: 8192 rows of 8 heads take 15.0 us, 3.4 TB/s, where
+// memory alone would take 7.9 us.  One trip to memory is all that the search and the
+// check for slots named twice add to the chain.  (Nine CTAs per SM: with the 63
+// registers that it would take unbounded eight fit, 13.40 us for 13.25 us on inputs that
+// are in part in L2.)
 __global__ void __launch_bounds__(APPEND_THREADS, 9) append_kernel(const AppendParams p) {
     constexpr uint32_t KEEP_TAIL = 1u << 31;
     __shared__ uint32_t s_max[4];                      // of a warp, and KEEP_TAIL
