@@ -104,6 +104,7 @@ struct Params {
     int32_t key_step;                  // from a key tile to the next: 128, or -128 (below)
     int32_t row_blocks;                // row_blocks * q_heads items, a CTA of the grid each
     int32_t block_rows;                // rows of an item: 256 or 128
+    int32_t ends_per_item;             // of cu_seqlens, to check
     int32_t ranked;                    // row blocks go by length, else from the last to the first
     int32_t wide_store;                // out rows are 32-byte aligned
     uint32_t negate;                   // scale < 0: the MMA negates Q, `scale` is positive
@@ -406,9 +407,12 @@ __device__ __forceinline__ int claimed_cta(uint32_t answer) {
     return got ? static_cast<int>(x) : -1;
 }
 
-// Reports document ends that do not start at 0, decrease or leave the call, by a whole warp.
-__device__ void check_cu_seqlens(const Params& p) {
-    for (int d = threadIdx.x & 31; d <= p.docs; d += 32) {
+// Reports document ends that do not start at 0, decrease or leave the call: item k's share
+// of them, by a whole warp.
+__device__ void check_cu_seqlens(const Params& p, int k) {
+    const int64_t first = static_cast<int64_t>(k) * p.ends_per_item;
+    const int64_t after = min(first + p.ends_per_item, static_cast<int64_t>(p.docs) + 1);
+    for (int64_t d = first + (threadIdx.x & 31); d < after; d += 32) {
         const int x = __ldg(p.cu_seqlens + d);
         const int before = d > 0 ? __ldg(p.cu_seqlens + d - 1) : 0;
         if (x < before || x > p.tokens || (d == 0 && x != 0))
@@ -439,9 +443,9 @@ __device__ void run_loads(const Params& p, uint8_t* smem, const Bars& b, volatil
     // for when this one's last loads are out.
     const uint32_t answer = smem_u32(smem + OFF_MISC + 16);
     const auto claim = [&]() {
-        // Once a call, with the first item: its CTA may have been taken over like any
-        // other.  Its loads are out, so nothing waits for this.
-        if (k == 0 && p.cu_seqlens != nullptr) check_cu_seqlens(p);
+        // With the items, which are all done by someone (any CTA, the first too, may have
+        // been taken over).  This one's loads are out, so nothing waits for it.
+        if (p.cu_seqlens != nullptr) check_cu_seqlens(p, k);
         if (lane == 0) {
             mbar_arrive_expect_tx(b.next, 16);
             claim_cta(answer, b.next);
@@ -1210,6 +1214,7 @@ extern "C" int fu_attention_forward(const fu_attention_args* a, uint32_t flags, 
     p.causal = a->causal;
     p.row_blocks = static_cast<int32_t>(row_blocks);
     p.block_rows = block_rows;
+    p.ends_per_item = static_cast<int32_t>(p.docs / blocks + 1);
     p.ranked = a->cu_seqlens != nullptr && p.row_blocks > 1 && p.row_blocks <= attention::MAX_RANKED;
     p.wide_store = (reinterpret_cast<uintptr_t>(a->out) | a->out_stride * 2) % 32 == 0;
     p.negate = a->scale < 0.f ? 1u : 0u;

@@ -463,8 +463,8 @@ struct Rows {
 // cap: up to a cap of FINE a small part of what rounding the weights to f16 costs.  Larger
 // caps matter for scores far below them, which take an odd polynomial of degree 7 in z, off
 // by 2e-7 with the slope at 0 exact: relative to the score it is off by less than 2^-19
-// (1.0e-6 and the roundings) whatever the cap.  (Both forms in one kernel: 34.8 us instead of 33.5 us for 256 sequences of up to
-// 1500 tokens with the first.)
+// (1.0e-6 and the roundings) whatever the cap.  (Both forms in one kernel: 34.8 us instead
+// of 33.5 us for 256 sequences of up to 1500 tokens with the first.)
 constexpr float FINE = 256.f;
 template <int kMode>
 struct Score {

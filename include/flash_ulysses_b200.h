@@ -351,7 +351,7 @@ typedef struct fu_attention_args {
     const void* q;                /* [tokens, q_heads * 128] */
     const void* k;                /* [tokens, kv_heads * 128] */
     const void* v;                /* [tokens, kv_heads * 128] */
-    void* out;                    /* [tokens, q_heads * 128] */
+    void* out;                    /* [tokens, q_heads * 128]; overlaps no input */
     int64_t q_stride, k_stride, v_stride, out_stride;
     const int32_t* cu_seqlens;    /* device, [docs + 1], or NULL: one document of all rows */
     const int32_t* prefix_lens;   /* device, [docs], or NULL; with causal only */
@@ -434,7 +434,7 @@ FU_API int64_t fu_kvcache_attention_workspace(int32_t device, int32_t q_heads, i
 /* out_i = attention of row i's query heads over the first seq_lens[i] tokens
  * of slot slots[i], the query being the last of them; scores as in
  * fu_attention_forward.  q and out are BF16 [seqs, q_heads * 128] with row
- * strides.  A row whose slot is negative is left as it was, one whose length
+ * strides, and do not overlap.  A row whose slot is negative is left as it was, one whose length
  * is 0 is zeroed.  A slot may occur more than once.  A slot outside the cache
  * or a length outside [0, max_blocks * 64] is reported and its row left as it
  * was; the keys of a block outside the cache are reported and not seen. */

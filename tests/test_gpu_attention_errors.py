@@ -1,5 +1,6 @@
-"""Attention calls whose document ends make no sense: reported whichever CTA does an item's work and
-whether the first item has rows or not, and the context works on once the error is cleared."""
+"""Attention calls whose document ends make no sense: reported wherever the entry lies, whichever CTA
+does an item's work and whether items have rows or not, and the context works on once the error is
+cleared."""
 
 import pytest
 
@@ -35,5 +36,28 @@ def test_many_documents_are_no_error():
     try:
         q, k, v = make(2000, 4, 1)
         check(ctx, q, k, v, 4, 1, cu=list(range(0, 2001)))
+    finally:
+        ctx.close()
+
+
+@pytest.mark.parametrize("n,heads,docs", [(4000, 4, 4000), (4000, 32, 4000), (40, 4, 3001),
+                                          (6000, 32, 11)])
+def test_one_bad_end_anywhere(n, heads, docs):
+    """A single entry below the one before it; there are more and fewer of them than items."""
+    ctx = make_context(heads, heads // 4)
+    try:
+        q, k, v = make(n, heads, heads // 4)
+        good = [n * d // docs for d in range(docs + 1)]
+        for at in sorted({1, 2, 31, 32, 33, docs // 2, docs - 1, docs}):
+            if not 0 < at <= docs:
+                continue
+            cu = list(good)
+            cu[at] = cu[at - 1] - 1
+            ctx.ulysses_attention_forward(q, k, v, cu_seqlens=ints(cu))
+            with pytest.raises(RuntimeError, match="cu_seqlens"):
+                ctx.check()
+            ctx.clear_error()
+        ctx.ulysses_attention_forward(q, k, v, cu_seqlens=ints(good))
+        ctx.check()
     finally:
         ctx.close()
